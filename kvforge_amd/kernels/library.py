@@ -56,6 +56,8 @@ MODULES: dict[str, list[str]] = {
     "ssm": ["ssm.hip"],
     "convkv": ["convkv.hip"],
     "chdelta": ["chdelta.hip"],
+    "beam": ["beam.hip"],
+    "attn_beams": ["attn_beams.hip"],
     "hostcheck": ["hostcheck.cpp"],
 }
 

@@ -1718,6 +1718,111 @@ def attn_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
           float(scale), sl, gp, gs, sk, cap, dp, nd, _stream()), "attn_mfma_decode")
 
 
+# ------------------------------------------------------------------------------ attention behind shared pages
+ATTN_BEAMS_MAX_CUTS = 64
+ATTN_BEAMS_KEYS_PER_CUT = 256
+
+
+def _here(who: str, first: torch.Tensor, *others) -> None:
+    """Launches go to the current device's stream: every operand lives there."""
+    at = first.device
+    if at.index != torch.cuda.current_device():
+        raise KernelError(f"{who}: operands live on {at}, the current device is {torch.cuda.current_device()}")
+    for t in others:
+        if t is not None and t.device != at:
+            raise KernelError(f"{who}: operands live on several devices")
+
+
+def attn_beams_takes(dtype: torch.dtype, head_dim: int) -> bool:
+    """Whether ``attn_beams`` has kernels for heads of this type and size."""
+    return dtype in (F32, BF16) and 0 < head_dim <= 256 and head_dim % 16 == 0
+
+
+def attn_beams_cuts(q: torch.Tensor, k_pages: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, num_groups: int,
+                    num_seqs: int, widest: int, max_shared: int, max_own: int) -> tuple[int, int]:
+    """(cuts of the keys that a group shares, cuts of a sequence's own keys) for ``attn_beams``: two workgroups a compute unit
+    where the keys suffice for cuts of ``ATTN_BEAMS_KEYS_PER_CUT``.  ``max_shared``, ``max_own``: the most shared keys of a
+    group and own keys of a sequence (any cuts give right results for any lengths)."""
+    room = 2 * compute_units(q.device)
+    rows = max(1, widest) * (num_heads // num_kv_heads)
+    tiles = int(_fn("attn_beams", "kvf_attn_beams_row_tiles", [c_int] * 3)(head_dim, k_pages.shape[2], rows))
+    shared = num_groups * num_kv_heads * -(-rows // (16 * tiles))
+
+    def cuts(groups: int, keys: int) -> int:
+        return max(1, min(-(-room // max(groups, 1)), -(-keys // ATTN_BEAMS_KEYS_PER_CUT), ATTN_BEAMS_MAX_CUTS))
+
+    return (cuts(shared, max_shared) if num_groups and max_shared > 0 else 0), cuts(num_seqs * num_kv_heads, max_own)
+
+
+def attn_beams_workspace(num_seqs: int, num_heads: int, head_dim: int, cuts: tuple[int, int], device
+                         ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Scratch of ``attn_beams``: the cuts' accumulators, and their (reference, sum) pairs."""
+    n = num_seqs * num_heads * (cuts[0] + cuts[1])
+    return torch.empty(n * head_dim, dtype=F32, device=device), torch.empty(n * 2, dtype=F32, device=device)
+
+
+def attn_beams(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, cu_groups: torch.Tensor,
+               shared_lens: torch.Tensor, ctx_lens: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_heads: int,
+               head_dim: int, scale: float, widest: int, cuts: tuple[int, int], workspace: tuple[torch.Tensor, torch.Tensor],
+               sinks: torch.Tensor | None = None) -> None:
+    """Attention of one token per sequence (row ``i`` of ``q`` is sequence ``i``'s) over ``ctx_lens[i]`` cached keys, for
+    sequences in groups ``cu_groups[g] .. cu_groups[g + 1] - 1`` whose first ``shared_lens[g]`` keys are the same, as the beams
+    of a request have them behind its prompt: these are read once for the whole group, from the pages of its first
+    sequence that holds any.  (Of a group's sequences that hold keys, none may be shorter than what is shared; where one is, its length counts
+    as shared.)  A sequence without keys gets zeros; one that no group names shares nothing.  Page numbers outside the
+    pages stand for keys that are not there.  ``widest``: sequences of the largest group (it decides how workgroups are laid out,
+    results do not depend on it).  ``cuts`` from ``attn_beams_cuts``, ``workspace`` from ``attn_beams_workspace``; launches that
+    share a workspace must not overlap.  ``sinks``: as in ``attn_prefill``.  Pages of any number of tokens (multiples of 8 are
+    loaded widely), heads of up to 256 elements in steps of 16."""
+    H, KV, d = num_heads, num_kv_heads, head_dim
+    if KV < 1 or H < 1 or H % KV:
+        raise KernelError(f"attn_beams: query heads ({H}) must be a multiple of kv heads ({KV})")
+    if not attn_beams_takes(q.dtype, d):
+        raise KernelError(f"attn_beams takes float32 or bfloat16 heads of up to 256 elements in steps of 16, got {q.dtype}, {d}")
+    _check(q, "q", None, (None, None), contiguous=False)
+    n = q.shape[0]
+    size = q.element_size()
+    if q.shape[1] < H * d or q.stride(1) != 1 or (n > 1 and q.stride(0) * size % 16) or q.data_ptr() % 16:
+        raise KernelError("attn_beams: rows of q hold all query heads, are dense and start on 16 bytes")
+    _check(k_pages, "k_pages", q.dtype, (None, KV, None, d))
+    nb, _, bs, _ = k_pages.shape
+    _check(v_pages, "v_pages", q.dtype, (nb, KV, d, bs))
+    if k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16 or nb < 1 or bs < 1:
+        raise KernelError("attn_beams: at least one page; pages start on 16 bytes")
+    _check(block_table, "block_table", I32, (n, None))
+    width = block_table.shape[1]
+    if width * bs >= 2**31 - 1024 or width * bs * bs >= 2**32:
+        raise KernelError(f"attn_beams: {width} pages of {bs} tokens a sequence are more than the kernel counts")
+    _check(cu_groups, "cu_groups", I32, (None,))
+    groups = cu_groups.shape[0] - 1
+    if groups < 0:
+        raise KernelError("attn_beams: cu_groups holds one more entry than there are groups")
+    _check(shared_lens, "shared_lens", I32, (groups,))
+    _check(ctx_lens, "ctx_lens", I32, (n,))
+    _check(out, "out", q.dtype, (n, H * d))
+    if out.data_ptr() % 16 or _overlap(out, q):
+        raise KernelError("attn_beams: out starts on 16 bytes and does not share memory with q")
+    cs, co = int(cuts[0]), int(cuts[1])
+    if not (0 <= cs <= ATTN_BEAMS_MAX_CUTS and 1 <= co <= ATTN_BEAMS_MAX_CUTS):
+        raise KernelError(f"attn_beams: up to {ATTN_BEAMS_MAX_CUTS} cuts of the shared keys and 1 to {ATTN_BEAMS_MAX_CUTS} of a "
+                          f"sequence's own, got {cs} and {co}")
+    if groups == 0:
+        cs = 0
+    if not 1 <= widest <= 1 << 15:
+        raise KernelError(f"attn_beams: the largest group has 1 to {1 << 15} sequences, got {widest}")
+    pa, pm = workspace
+    _check(pa, "workspace[0]", F32, (None,))
+    _check(pm, "workspace[1]", F32, (None,))
+    if pa.shape[0] < n * H * (cs + co) * d or pm.shape[0] < n * H * (cs + co) * 2 or pa.data_ptr() % 16:
+        raise KernelError("attn_beams: workspace too small")
+    sk = _sinks_ptr(sinks, H, q)
+    _here("attn_beams", q, k_pages, v_pages, block_table, cu_groups, shared_lens, ctx_lens, out, pa, pm)
+    f = _fn("attn_beams", "kvf_attn_beams", [c_int] + [c_void_p] * 11 + [c_int] * 13 + [c_float, c_void_p])
+    _ok(f(_tcode(q.dtype), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), cu_groups.data_ptr(),
+          shared_lens.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), pa.data_ptr(), pm.data_ptr(), sk, H, KV, d, bs, nb, width,
+          q.stride(0) if n > 1 else H * d, H * d, n, groups, int(widest), cs, co, float(scale), _stream()), "attn_beams")
+
+
 # ------------------------------------------------------------------------------ matrix-memory recurrence
 MLSTM_CHUNK_FROM = 8     # runs of at least so many tokens go chunk by chunk on the matrix cores
 MLSTM_MULTI_FROM = 192   # and runs of at least so many through the passes that take all chunks at once
@@ -2772,3 +2877,126 @@ def decode_advance(sampled: torch.Tensor, token_ids: torch.Tensor, positions: to
     _ok(f(sampled.data_ptr(), token_ids.data_ptr(), positions.data_ptr(), ctx_lens.data_ptr(),
           ring.data_ptr(), counter.data_ptr(), r, ring.shape[1], ring.shape[0], _stream()),
         "decode_advance")
+
+
+# ------------------------------------------------------------------------------ beam search
+BEAM_MAX_COUNT = 64      # candidates of a request
+BEAM_MAX_WIDTH = 32      # beams of a request that are reordered together
+BEAM_PIECES = (2048, 8192)     # logits of a row that one workgroup takes
+
+
+def _beam_pieces(rows: int, vocab: int, count: int, device) -> tuple[int, int]:
+    """(pieces of a row, logits of a piece): large pieces where they give every compute unit two workgroups."""
+    small, large = BEAM_PIECES
+    most = vocab + 7           # a row may begin inside its first 16 bytes
+    piece = large if count <= 32 and rows * -(-most // large) >= 2 * compute_units(device) else small
+    return -(-most // piece), piece
+
+
+def beam_select_workspace(rows: int, vocab: int, count: int, device) -> tuple[torch.Tensor, ...]:
+    """Scratch of ``beam_select`` for ``rows`` rows of logits: the pieces' sums and the rows', the pieces' best logits and
+    their tokens."""
+    pieces, _ = _beam_pieces(rows, vocab, count, device)
+    return (torch.empty(rows * pieces * 2, dtype=torch.float64, device=device),
+            torch.empty(rows * 2, dtype=torch.float64, device=device),
+            torch.empty(rows * pieces * count, dtype=F32, device=device),
+            torch.empty(rows * pieces * count, dtype=I32, device=device))
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, cu_beams: torch.Tensor, out_scores: torch.Tensor,
+                out_beams: torch.Tensor, out_tokens: torch.Tensor, workspace: tuple[torch.Tensor, ...]) -> None:
+    """The best continuations of every request: of all its beams (rows ``cu_beams[r] .. cu_beams[r + 1] - 1`` of ``logits``, fp32
+    or bf16) and tokens, the ``out_scores.shape[1]`` with the largest ``scores[beam] + log_softmax(logits[beam])[token]``, best
+    first (compared in 64 bits), equal ones by the lower beam, then the larger logit, then the lower token.  ``out_beams`` counts from the request's first beam.  Beams whose
+    score is not finite have ended and give none; tokens whose logit is NaN or -inf are ruled out (``+inf`` counts as the
+    largest finite number).  Where there are fewer candidates, the rest is (-inf, -1, -1).  ``workspace`` from
+    ``beam_select_workspace``; launches that share one must not overlap."""
+    if logits.dtype not in (F32, BF16):
+        raise KernelError(f"beam_select takes float32 or bfloat16 logits, got {logits.dtype}")
+    _check(logits, "logits", None, (None, None), contiguous=False)
+    rows, vocab = logits.shape
+    if vocab < 1 or logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
+        raise KernelError("beam_select: rows of logits are dense and do not overlap")
+    if rows > 65535 or vocab > 2**30:
+        raise KernelError(f"beam_select takes up to 65535 rows of up to 2^30 logits, got {rows} of {vocab}")
+    _check(scores, "scores", F32, (rows,))
+    _check(cu_beams, "cu_beams", I32, (None,))
+    requests = cu_beams.shape[0] - 1
+    if requests < 0:
+        raise KernelError("beam_select: cu_beams holds one more entry than there are requests")
+    _check(out_scores, "out_scores", F32, (requests, None))
+    count = out_scores.shape[1]
+    if not 1 <= count <= BEAM_MAX_COUNT:
+        raise KernelError(f"beam_select gives 1 to {BEAM_MAX_COUNT} candidates a request, asked for {count}")
+    _check(out_beams, "out_beams", I32, (requests, count))
+    _check(out_tokens, "out_tokens", I32, (requests, count))
+    if any(_overlap(o, i) for o in (out_scores, out_beams, out_tokens) for i in (scores, logits, cu_beams)):
+        raise KernelError("beam_select: outputs do not share memory with inputs")
+    pieces, piece = _beam_pieces(rows, vocab, count, logits.device)
+    if pieces * count > 65536 or rows * pieces * count >= 2**31:
+        raise KernelError(f"beam_select: {count} candidates of each of {pieces} pieces of {rows} rows are more than the kernel counts")
+    sums, row_of, values, tokens = workspace
+    _check(sums, "workspace[0]", torch.float64, (None,))
+    _check(row_of, "workspace[1]", torch.float64, (None,))
+    _check(values, "workspace[2]", F32, (None,))
+    _check(tokens, "workspace[3]", I32, (None,))
+    if (sums.shape[0] < rows * pieces * 2 or row_of.shape[0] < rows * 2
+            or min(values.shape[0], tokens.shape[0]) < rows * pieces * count or sums.data_ptr() % 16 or row_of.data_ptr() % 16):
+        raise KernelError("beam_select: workspace too small for these rows, logits and candidates")
+    _here("beam_select", logits, scores, cu_beams, out_scores, out_beams, out_tokens, *workspace)
+    f = _fn("beam", "kvf_beam_select", [c_int, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 8)
+    _ok(f(_tcode(logits.dtype), logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, scores.data_ptr(),
+          cu_beams.data_ptr(), requests, count, pieces, piece, sums.data_ptr(), row_of.data_ptr(), values.data_ptr(),
+          tokens.data_ptr(), out_scores.data_ptr(), out_beams.data_ptr(), out_tokens.data_ptr(), _stream()), "beam_select")
+
+
+class CacheRows:
+    """Tensors whose rows (pages, or state slots, of every layer) move together: ``beam_reorder`` moves the same rows in all
+    of them with one launch.  Rows are dense; they may be columns of wider ones.  Keeps the tensors, and a table of them on
+    their device."""
+
+    def __init__(self, tensors) -> None:
+        self.tensors = list(tensors)
+        if not self.tensors:
+            raise KernelError("CacheRows: at least one tensor")
+        first = self.tensors[0]
+        spans, table, tiles = [], [], []
+        tile_bytes = int(_fn("beam", "kvf_beam_tile_bytes", [])())
+        for t in self.tensors:
+            _check(t, "tensor", None, None, contiguous=False)
+            if t.dim() < 2 or t.shape[0] != first.shape[0] or t.device != first.device or t.numel() == 0:
+                raise KernelError("CacheRows: tensors [rows, ...] with as many rows, on one device")
+            size, row = t.element_size(), t[0].numel() * t.element_size()
+            stride = t.stride(0) * size if t.shape[0] > 1 else row
+            if not t[0].is_contiguous() or stride < row or size % 2:
+                raise KernelError("CacheRows: rows are dense, do not overlap, and have elements of two bytes or more")
+            at = t.data_ptr()
+            behind = (t.shape[0] - 1) * stride
+            for a, s, b in spans:
+                if (a < at + behind + row and at < a + (t.shape[0] - 1) * s + b
+                        and (s != stride or (at - a) % s < b or (a - at) % s < row)):
+                    raise KernelError("CacheRows: rows of different tensors share memory")
+            spans.append((at, stride, row))
+            unit = next(u for u in (16, 8, 4, 2) if at % u == 0 and stride % u == 0 and row % u == 0)
+            table.append((at, stride, row, unit))
+            tiles.append(-(-row // tile_bytes))
+        self.rows, self.device = int(first.shape[0]), first.device
+        self.table = torch.tensor(table, dtype=torch.int64, device=self.device)
+        self.tiles = torch.cat([torch.stack([torch.full((n,), i, dtype=I32), torch.arange(n, dtype=I32)], dim=1)
+                                for i, n in enumerate(tiles)]).contiguous().to(self.device)
+
+
+def beam_reorder(rows: CacheRows, slots: torch.Tensor, parents: torch.Tensor) -> None:
+    """What beams own follows the beams that were selected: of every request ``r`` (``slots``, ``parents``: int32
+    ``[requests, beams]``) and beam ``b``, row ``slots[r, b]`` of every tensor becomes what row ``slots[r, parents[r, b]]`` was
+    before the call.  Beams that go on from themselves stay; entries outside the rows, or outside the request's beams, move
+    nothing.  The slots of a call are distinct."""
+    _check(slots, "slots", I32, (None, None))
+    requests, beams = slots.shape
+    _check(parents, "parents", I32, (requests, beams))
+    if not 1 <= beams <= BEAM_MAX_WIDTH or requests > 65535:
+        raise KernelError(f"beam_reorder takes up to 65535 requests of 1 to {BEAM_MAX_WIDTH} beams, got {requests} of {beams}")
+    _here("beam_reorder", rows.table, slots, parents)
+    f = _fn("beam", "kvf_beam_reorder", [c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 3)
+    _ok(f(rows.table.data_ptr(), rows.tiles.data_ptr(), rows.tiles.shape[0], rows.rows, requests, beams, slots.data_ptr(),
+          parents.data_ptr(), _stream()), "beam_reorder")

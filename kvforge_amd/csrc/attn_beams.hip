@@ -28,6 +28,9 @@ constexpr int BLOCK = 32;              // keys a wave takes at a time
 constexpr float LAZY = 8.f;
 constexpr float LOG2E = 1.4426950408889634f;
 
+// Where two waves a SIMD are asked for, a wave has at most 256 registers.
+#define KVF_TWO_WAVES(FITS) __attribute__((amdgpu_waves_per_eu((FITS) ? 2 : 1)))
+
 struct Args {
   int H, KV, d, bs, nb, width, q_stride, o_stride, n_seqs, n_groups;
   int blocks;          // row blocks of a group that have a workgroup of their own
@@ -115,228 +118,259 @@ __device__ __forceinline__ int shared_keys(int group, int first, int n, const in
   return max(0, min(least, shared_lens[group]));
 }
 
-// Rows [row0, row0 + 16 RT) of `rows` (sequence first + row / G, head row % G of kv head `kvh`), keys [lo, hi) of the pages in
-// `table`; results go to cut `cut`.  DT: tiles of 16 elements of d (at least d / 16).
-template <typename T, int DT, int RT, bool ALIGNED>
-__device__ void attend(const Tensors<T>& t, const Args& a, const int* __restrict__ table, int first, int rows, int row0, int kvh,
-                       int lo, int hi, int cut, f32x4* lds_acc, float2* lds_ml) {
+// What a wave holds of 16 * RT rows: Q, and the running reference, sum and accumulator of each.
+template <typename T, int DT, int RT> struct Rows {
   typedef Frag<T> F;
-  constexpr int SLICES = DT * 16 / F::SLICE, LANE_D = F::SLICE / 4;
-  const int lane = threadIdx.x % KVF_WAVE, wave = threadIdx.x / KVF_WAVE, g = lane / 16, r = lane % 16;
-  const int G = a.H / a.KV, d = a.d, tiles = d / 16;
+  static constexpr int SLICES = DT * 16 / F::SLICE, LANE_D = F::SLICE / 4;
   typename F::Part q[RT][SLICES];
-  bool live[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int row = row0 + rt * 16 + r;
-    const int seq = first + min(row, rows - 1) / G;
-    live[rt] = row < rows && t.ctx_lens[seq] > 0;
-    const T* from = t.q + static_cast<long>(seq) * a.q_stride + (kvh * G + min(row, rows - 1) % G) * d;
-#pragma unroll
-    for (int c = 0; c < SLICES; ++c) {
-      const int e = c * F::SLICE + g * LANE_D;
-      q[rt][c] = e < d ? F::load(from + e) : F::zero();
-    }
-  }
   f32x4 acc[RT][DT];
   float m[RT], sum[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -INFINITY;
-    sum[rt] = 0.f;
-#pragma unroll
-    for (int j = 0; j < DT; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  const long page_elems = static_cast<long>(a.KV) * a.bs * d;
-  const T* kp = t.k + static_cast<long>(kvh) * a.bs * d;
-  const T* vp = t.v + static_cast<long>(kvh) * a.bs * d;
-  // page numbers of the eight keys from `key` on (ALIGNED: one page), 0 and a cleared bit where there is none
-  auto lookup = [&](int key, bool& ok) {
-    const int p = key >= lo - 7 && key < hi ? table[page_of(key, a)] : -1;
-    ok = p >= 0 && p < a.nb;
-    return ok ? p : 0;
-  };
-  for (int kb = (lo & ~7) + wave * BLOCK; kb < hi; kb += WAVES * BLOCK) {
-    typename F::Part kf[2][SLICES];
-    typename F::Keys vf[DT];
-    unsigned keep = 0;                // which of the lane's keys 8 g .. 8 g + 7 count
-    if constexpr (ALIGNED) {
-      bool ok_k, ok_v;
-      const int key_k = kb + 8 * (r / 4), key_v = kb + 8 * g;
-      const int pk = lookup(key_k, ok_k), pv = lookup(key_v, ok_v);
-      const int off_k = ok_k ? key_k - page_of(key_k, a) * a.bs : 0, off_v = ok_v ? key_v - page_of(key_v, a) * a.bs : 0;
-      const T* k0 = kp + pk * page_elems + static_cast<long>(off_k + r % 4) * d;
-      const T* v0 = vp + pv * page_elems + off_v + r * a.bs;
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int c = 0; c < SLICES; ++c) {
-          const int e = c * F::SLICE + g * LANE_D;
-          kf[tt][c] = e < d ? F::load(k0 + tt * 4 * d + e) : F::zero();
-        }
-#pragma unroll
-      for (int j = 0; j < DT; ++j)
-        if (j < tiles) vf[j] = F::load_keys(v0 + static_cast<long>(j) * 16 * a.bs);
-      const int from = max(lo - key_v, 0), to = min(hi - key_v, 8);
-      keep = ok_v && to > from ? (0xffu >> (8 - to)) & (0xffu << from) : 0u;
-    } else {
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        const int key = kb + 8 * (r / 4) + 4 * tt + r % 4;
-        bool ok = false;
-        int p = 0, off = 0;
-        if (key >= lo && key < hi) {
-          p = table[key / a.bs];
-          ok = p >= 0 && p < a.nb;
-          off = key % a.bs;
-        }
-        const T* k0 = kp + (ok ? p : 0) * page_elems + static_cast<long>(ok ? off : 0) * d;
-#pragma unroll
-        for (int c = 0; c < SLICES; ++c) {
-          const int e = c * F::SLICE + g * LANE_D;
-          kf[tt][c] = e < d ? F::load(k0 + e) : F::zero();
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int key = kb + 8 * g + i;
-        bool ok = false;
-        int p = 0, off = 0;
-        if (key >= lo && key < hi) {
-          p = table[key / a.bs];
-          ok = p >= 0 && p < a.nb;
-          off = key % a.bs;
-        }
-        keep |= ok ? 1u << i : 0u;
-        const T* v0 = vp + (ok ? p : 0) * page_elems + (ok ? off : 0) + r * a.bs;
-#pragma unroll
-        for (int j = 0; j < DT; ++j)
-          if (j < tiles) F::set(vf[j], i, v0[static_cast<long>(j) * 16 * a.bs]);
-      }
-    }
-    const bool whole = __all(keep == 0xffu);
-    if (!whole)
-#pragma unroll
-      for (int j = 0; j < DT; ++j)
-        if (j < tiles) F::clear(vf[j], keep);
+
+  // Rows [row0, row0 + 16 RT) of `rows`: sequence first + row / G, head row % G of kv head `kvh`.
+  __device__ __forceinline__ void start(const Tensors<T>& t, const Args& a, int first, int rows, int row0, int kvh) {
+    const int lane = threadIdx.x % KVF_WAVE, g = lane / 16, r = lane % 16, G = a.H / a.KV;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      f32x4 s[2];
+      const int row = min(row0 + rt * 16 + r, rows - 1);
+      const T* from = t.q + static_cast<long>(first + row / G) * a.q_stride + (kvh * G + row % G) * a.d;
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        s[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < SLICES; ++c) s[tt] = F::scores(kf[tt][c], q[rt][c], s[tt]);
-        s[tt] *= a.scale2;
-        if (!whole)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[tt][i] = keep >> (4 * tt + i) & 1u ? s[tt][i] : -INFINITY;
+      for (int c = 0; c < SLICES; ++c) {
+        const int e = c * F::SLICE + g * LANE_D;
+        q[rt][c] = e < a.d ? F::load(from + e) : F::zero();
       }
-      float most = s[0][0];
+      m[rt] = -INFINITY;
+      sum[rt] = 0.f;
 #pragma unroll
-      for (int i = 1; i < 8; ++i) most = fmaxf(most, s[i / 4][i % 4]);
-      if (__any(most > m[rt] + LAZY)) {
-        most = fmaxf(most, __shfl_xor(most, 16, KVF_WAVE));
-        most = fmaxf(most, __shfl_xor(most, 32, KVF_WAVE));
-        const float raised = fmaxf(m[rt], most);
-        const float by = raised > -INFINITY ? __builtin_amdgcn_exp2f(m[rt] - raised) : 1.f;
-        m[rt] = raised;
-        sum[rt] *= by;
-#pragma unroll
-        for (int j = 0; j < DT; ++j) acc[rt][j] *= by;
-      }
-      const float ref = m[rt] > -INFINITY ? m[rt] : 0.f;
-      f32x4 p[2];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i / 4][i % 4] = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - ref);
-        sum[rt] += p[i / 4][i % 4];
-      }
-      const typename F::Probs pf = F::probs(p);
-#pragma unroll
-      for (int j = 0; j < DT; ++j)
-        if (j < tiles) acc[rt][j] = F::values(vf[j], pf, acc[rt][j]);
+      for (int j = 0; j < DT; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
-  // the waves' results, one tile of rows at a time
+
+  // Blocks kb, kb + step, ... of the keys [lo, hi) of the pages in `table`.  kb: a multiple of 8.  The page numbers of a
+  // block are looked up, and its K fragments loaded, while the block before it is worked on.
+  template <bool ALIGNED>
+  __device__ __forceinline__ void walk(const Tensors<T>& t, const Args& a, const int* __restrict__ table, int kvh, int kb, int step, int lo, int hi) {
+    const int lane = threadIdx.x % KVF_WAVE, g = lane / 16, r = lane % 16;
+    const int d = a.d, tiles = d / 16;
+    const long page_elems = static_cast<long>(a.KV) * a.bs * d;
+    const T* kp = t.k + static_cast<long>(kvh) * a.bs * d;
+    const T* vp = t.v + static_cast<long>(kvh) * a.bs * d;
+    typename F::Part kf[2][SLICES];
+    // the page that holds the keys from `key` on, -1 where there is none
+    auto lookup = [&](int key) { return key < hi ? table[page_of(key, a)] : -1; };
+    auto valid = [&](int page) { return page >= 0 && page < a.nb; };
+    auto load_k = [&](int at, int page) {         // ALIGNED: the page of keys at + 8 (r / 4)
+      if constexpr (ALIGNED) {
+        const int key = at + 8 * (r / 4);
+        const bool ok = valid(page);
+        const T* from = kp + (ok ? page : 0) * page_elems + static_cast<long>((ok ? key - page_of(key, a) * a.bs : 0) + r % 4) * d;
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    float l = sum[rt];
-    l += __shfl_xor(l, 16, KVF_WAVE);
-    l += __shfl_xor(l, 32, KVF_WAVE);
-    __syncthreads();
-    if (g == 0) lds_ml[wave * 16 + r] = make_float2(m[rt], l);
-    __syncthreads();
-    float top = -INFINITY, total = 0.f;
+        for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, lds_ml[w * 16 + r].x);
+          for (int c = 0; c < SLICES; ++c) {
+            const int e = c * F::SLICE + g * LANE_D;
+            kf[tt][c] = e < d ? F::load(from + tt * 4 * d + e) : F::zero();
+          }
+      } else {
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float2 o = lds_ml[w * 16 + r];
-      total += o.x > -INFINITY || o.y != o.y ? o.y * __builtin_amdgcn_exp2f(o.x - top) : 0.f;     // (NaN stays NaN)
-    }
-    const float by = m[rt] > -INFINITY ? __builtin_amdgcn_exp2f(m[rt] - top) : 0.f;
+        for (int tt = 0; tt < 2; ++tt) {
+          const int key = at + 8 * (r / 4) + 4 * tt + r % 4;
+          const int p = key < hi ? table[key / a.bs] : -1;
+          const T* from = kp + (valid(p) ? p : 0) * page_elems + static_cast<long>(valid(p) ? key % a.bs : 0) * d;
 #pragma unroll
-    for (int j = 0; j < DT; ++j) {
-      acc[rt][j] *= by;
-      if (wave > 0 && j < tiles) lds_acc[((wave - 1) * DT + j) * KVF_WAVE + lane] = acc[rt][j];
-    }
-    __syncthreads();
-    if (wave == 0) {
-#pragma unroll
-      for (int j = 0; j < DT; ++j)
-        if (j < tiles) {
-          f32x4 o = acc[rt][j];
-#pragma unroll
-          for (int w = 0; w < WAVES - 1; ++w) o += lds_acc[(w * DT + j) * KVF_WAVE + lane];
-          acc[rt][j] = o;
+          for (int c = 0; c < SLICES; ++c) {
+            const int e = c * F::SLICE + g * LANE_D;
+            kf[tt][c] = e < d ? F::load(from + e) : F::zero();
+          }
         }
-      const int row = row0 + rt * 16 + r;
-      if (row < rows) {
-        const int seq = first + row / G, h = kvh * G + row % G;
-        const long at = (static_cast<long>(seq) * a.H + h) * (a.cs + a.co) + cut;
-        const bool any = live[rt] && (total > 0.f || total != total);
-        if (g == 0) t.ml[at] = any ? make_float2(top > -INFINITY ? top : 0.f, total) : make_float2(-INFINITY, 0.f);
-        if (any)
+      }
+    };
+    if (kb >= hi) return;
+    int pv = 0;                          // ALIGNED: the page of keys kb + 8 g
+    if constexpr (ALIGNED) {
+      const int pk = lookup(kb + 8 * (r / 4));
+      pv = lookup(kb + 8 * g);
+      load_k(kb, pk);
+    } else {
+      load_k(kb, 0);
+    }
+    while (true) {
+      const int next = kb + step;
+      typename F::Keys vf[DT];
+      unsigned keep = 0;                // which of the lane's keys kb + 8 g + (0 .. 7) count
+      int pk_next = -1, pv_next = -1;
+      if constexpr (ALIGNED) {
+        const int key = kb + 8 * g, from = max(lo - key, 0), to = min(hi - key, 8);
+        const bool ok = valid(pv);
+        keep = ok && to > from ? (0xffu >> (8 - to)) & (0xffu << from) : 0u;
+        const T* v0 = vp + (ok ? pv : 0) * page_elems + (ok ? key - page_of(key, a) * a.bs : 0) + r * a.bs;
+#pragma unroll
+        for (int j = 0; j < DT; ++j)
+          if (j < tiles) vf[j] = F::load_keys(v0 + static_cast<long>(j) * 16 * a.bs);
+        pk_next = lookup(next + 8 * (r / 4));
+        pv_next = lookup(next + 8 * g);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = kb + 8 * g + i;
+          const int p = key >= lo && key < hi ? table[key / a.bs] : -1;
+          keep |= valid(p) ? 1u << i : 0u;
+          const T* v0 = vp + (valid(p) ? p : 0) * page_elems + (valid(p) ? key % a.bs : 0) + r * a.bs;
 #pragma unroll
           for (int j = 0; j < DT; ++j)
-            if (j < tiles) *reinterpret_cast<f32x4*>(t.acc + at * d + j * 16 + g * 4) = acc[rt][j];
+            if (j < tiles) F::set(vf[j], i, v0[static_cast<long>(j) * 16 * a.bs]);
+        }
       }
+      const bool whole = __all(keep == 0xffu);
+      f32x4 s[RT][2];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+          s[rt][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < SLICES; ++c) s[rt][tt] = F::scores(kf[tt][c], q[rt][c], s[rt][tt]);
+        }
+      if (next < hi) load_k(next, pk_next);
+      typename F::Probs pf[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+          s[rt][tt] *= a.scale2;
+          if (!whole)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[rt][tt][i] = keep >> (4 * tt + i) & 1u ? s[rt][tt][i] : -INFINITY;
+        }
+        float most = s[rt][0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) most = fmaxf(most, s[rt][i / 4][i % 4]);
+        if (__any(most > m[rt] + LAZY)) {
+          most = fmaxf(most, __shfl_xor(most, 16, KVF_WAVE));
+          most = fmaxf(most, __shfl_xor(most, 32, KVF_WAVE));
+          const float raised = fmaxf(m[rt], most);
+          const float by = raised > -INFINITY ? __builtin_amdgcn_exp2f(m[rt] - raised) : 1.f;
+          m[rt] = raised;
+          sum[rt] *= by;
+#pragma unroll
+          for (int j = 0; j < DT; ++j) acc[rt][j] *= by;
+        }
+        const float ref = m[rt] > -INFINITY ? m[rt] : 0.f;
+        f32x4 p[2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[i / 4][i % 4] = __builtin_amdgcn_exp2f(s[rt][i / 4][i % 4] - ref);
+          sum[rt] += p[i / 4][i % 4];
+        }
+        pf[rt] = F::probs(p);
+      }
+      if (!whole)
+#pragma unroll
+        for (int j = 0; j < DT; ++j)
+          if (j < tiles) F::clear(vf[j], keep);
+#pragma unroll
+      for (int j = 0; j < DT; ++j)
+        if (j < tiles)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) acc[rt][j] = F::values(vf[j], pf[rt], acc[rt][j]);
+      if (next >= hi) break;
+      kb = next;
+      pv = pv_next;
+      if constexpr (!ALIGNED) (void)pk_next;
     }
   }
-}
 
-// Cut `c` of `n` of the keys [lo, hi), in whole rounds of the waves.
-__device__ __forceinline__ void cut_of(int& lo, int& hi, int c, int n) {
-  const int first = lo & ~7, round = WAVES * BLOCK;
+  // Leaves tile rt's results as cut `cut` of its rows (`total`: sums over all keys of the cut).
+  __device__ __forceinline__ void leave(const Tensors<T>& t, const Args& a, int rt, float top, float total, int first, int rows, int row0, int kvh, int cut) {
+    const int lane = threadIdx.x % KVF_WAVE, g = lane / 16, r = lane % 16, G = a.H / a.KV, tiles = a.d / 16;
+    const int row = row0 + rt * 16 + r;
+    if (row >= rows) return;
+    const int seq = first + row / G;
+    const long at = (static_cast<long>(seq) * a.H + kvh * G + row % G) * (a.cs + a.co) + cut;
+    const bool any = t.ctx_lens[seq] > 0 && (total > 0.f || total != total);      // (NaN stays NaN)
+    if (g == 0) t.ml[at] = any ? make_float2(top > -INFINITY ? top : 0.f, total) : make_float2(-INFINITY, 0.f);
+    if (any)
+#pragma unroll
+      for (int j = 0; j < DT; ++j)
+        if (j < tiles) *reinterpret_cast<f32x4*>(t.acc + at * a.d + j * 16 + g * 4) = acc[rt][j];
+  }
+  __device__ __forceinline__ float whole_sum(int rt) const {
+    float l = sum[rt];
+    l += __shfl_xor(l, 16, KVF_WAVE);
+    return l + __shfl_xor(l, 32, KVF_WAVE);
+  }
+};
+
+// Cut `c` of `n` of the keys [lo, hi), in whole rounds of `round` keys.
+__device__ __forceinline__ void cut_of(int& lo, int& hi, int c, int n, int round) {
+  const int first = lo & ~7;
   const int per = ((hi - first + n - 1) / n + round - 1) / round * round;
   const int from = first + min(c * per, hi - first), to = min(from + per, hi);
   lo = max(lo, from);
   hi = to;
 }
 
+// The workgroups of the first n_groups * cs * blocks * KV numbers take a cut of a group's shared keys, the four waves a block
+// each in turn; of the others every wave takes a cut of a sequence's own keys by itself.  The kv head is the fastest index:
+// workgroups go to the eight XCDs in turn, so with eight heads an L2 holds the keys of one, also for a group's further rows.
 template <typename T, int DT, int RT, bool ALIGNED>
-__global__ __launch_bounds__(THREADS) void attn_beams_kernel(Tensors<T> t, Args a) {
+__global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 16 && DT < 16 : RT * DT <= 8) void attn_beams_kernel(Tensors<T> t, Args a) {
   __shared__ f32x4 lds_acc[(WAVES - 1) * DT * KVF_WAVE];
   __shared__ float2 lds_ml[WAVES * 16];
   const int shared_items = a.n_groups * a.cs * a.blocks * a.KV;
-  const int G = a.H / a.KV, most = a.width * a.bs, lane = threadIdx.x % KVF_WAVE;
-  int item = blockIdx.x;
-  if (item < shared_items) {
+  const int G = a.H / a.KV, most = a.width * a.bs, lane = threadIdx.x % KVF_WAVE, wave = threadIdx.x / KVF_WAVE, r = lane % 16;
+  if (static_cast<int>(blockIdx.x) < shared_items) {
+    const int item = blockIdx.x;
     const int kvh = item % a.KV, block = item / a.KV % a.blocks, cut = item / a.KV / a.blocks % a.cs, group = item / a.KV / a.blocks / a.cs;
     const int first = min(max(t.cu_groups[group], 0), a.n_seqs), n = min(max(t.cu_groups[group + 1], first), a.n_seqs) - first;
     if (n == 0) return;
+    const int rows = n * G, tiles = a.d / 16;
     int holder, lo = 0, hi = shared_keys(group, first, n, t.shared_lens, t.ctx_lens, most, holder);
-    cut_of(lo, hi, cut, a.cs);
-    for (int row0 = block * 16 * RT; row0 < n * G; row0 += a.blocks * 16 * RT)
-      attend<T, DT, RT, ALIGNED>(t, a, t.table + static_cast<long>(holder) * a.width, first, n * G, row0, kvh, lo, hi, cut, lds_acc, lds_ml);
+    cut_of(lo, hi, cut, a.cs, WAVES * BLOCK);
+    for (int row0 = block * 16 * RT; row0 < rows; row0 += a.blocks * 16 * RT) {
+      Rows<T, DT, RT> x;
+      x.start(t, a, first, rows, row0, kvh);
+      x.template walk<ALIGNED>(t, a, t.table + static_cast<long>(holder) * a.width, kvh, lo + wave * BLOCK, WAVES * BLOCK, lo, hi);
+      // the waves' results, one tile of rows at a time
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float l = x.whole_sum(rt);
+        __syncthreads();
+        if (lane < 16) lds_ml[wave * 16 + r] = make_float2(x.m[rt], l);
+        __syncthreads();
+        float top = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, lds_ml[w * 16 + r].x);
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+          const float2 o = lds_ml[w * 16 + r];
+          total += o.x > -INFINITY || o.y != o.y ? o.y * __builtin_amdgcn_exp2f(o.x - top) : 0.f;
+        }
+        const float by = x.m[rt] > -INFINITY ? __builtin_amdgcn_exp2f(x.m[rt] - top) : 0.f;
+#pragma unroll
+        for (int j = 0; j < DT; ++j) {
+          x.acc[rt][j] *= by;
+          if (wave > 0 && j < tiles) lds_acc[((wave - 1) * DT + j) * KVF_WAVE + lane] = x.acc[rt][j];
+        }
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+          for (int j = 0; j < DT; ++j)
+            if (j < tiles)
+#pragma unroll
+              for (int w = 0; w < WAVES - 1; ++w) x.acc[rt][j] += lds_acc[(w * DT + j) * KVF_WAVE + lane];
+          x.leave(t, a, rt, top, total, first, rows, row0, kvh, cut);
+        }
+      }
+    }
   } else {
-    item -= shared_items;
+    // (no barrier from here on)
+    const int item = (blockIdx.x - shared_items) * WAVES + wave;
     const int kvh = item % a.KV, cut = item / a.KV % a.co, seq = item / a.KV / a.co;
+    if (seq >= a.n_seqs) return;
     // the group that the sequence is in
     int lo = 0;
     bool grouped = false;
-    for (int g0 = 0; g0 < a.n_groups; g0 += KVF_WAVE) {
+    for (int g0 = 0; g0 < a.n_groups && !grouped; g0 += KVF_WAVE) {
       const int g = min(g0 + lane, a.n_groups - 1);
       const unsigned long long here = __ballot(t.cu_groups[g] <= seq && seq < t.cu_groups[g + 1]);
       if (here) {
@@ -345,16 +379,19 @@ __global__ __launch_bounds__(THREADS) void attn_beams_kernel(Tensors<T> t, Args 
         int holder;
         lo = a.cs ? shared_keys(group, first, min(t.cu_groups[group + 1], a.n_seqs) - first, t.shared_lens, t.ctx_lens, most, holder) : 0;
         grouped = true;
-        break;
       }
     }
     if (!grouped && cut == 0)       // nobody else tells of its shared keys
-      for (int i = threadIdx.x; i < G * a.cs; i += THREADS)
+      for (int i = lane; i < G * a.cs; i += KVF_WAVE)
         t.ml[(static_cast<long>(seq) * a.H + kvh * G + i / a.cs) * (a.cs + a.co) + i % a.cs] = make_float2(-INFINITY, 0.f);
     int hi = max(lo, min(t.ctx_lens[seq], most));
-    cut_of(lo, hi, cut, a.co);
-    for (int row0 = 0; row0 < G; row0 += 16 * RT)
-      attend<T, DT, RT, ALIGNED>(t, a, t.table + static_cast<long>(seq) * a.width, seq, G, row0, kvh, lo, hi, a.cs + cut, lds_acc, lds_ml);
+    cut_of(lo, hi, cut, a.co, BLOCK);
+    for (int row0 = 0; row0 < G; row0 += 16) {
+      Rows<T, DT, 1> x;
+      x.start(t, a, seq, G, row0, kvh);
+      x.template walk<ALIGNED>(t, a, t.table + static_cast<long>(seq) * a.width, kvh, lo & ~7, BLOCK, lo, hi);
+      x.leave(t, a, 0, x.m[0], x.whole_sum(0), seq, G, row0, kvh, a.cs + cut);
+    }
   }
 }
 
@@ -381,11 +418,24 @@ __global__ __launch_bounds__(THREADS) void attn_beams_join_kernel(const float* _
   const int quads = a.d / 4, side = quads > 32 ? 1 : quads > 16 ? 2 : 4;
   const int sub = lane / (KVF_WAVE / side), at = lane % (KVF_WAVE / side);
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (at < quads)
-    for (int c = sub; c < cuts; c += side) {
-      const float2 x = mine[c];
-      if (x.x > -INFINITY) o += *reinterpret_cast<const f32x4*>(acc + (row * cuts + c) * a.d + at * 4) * __builtin_amdgcn_exp2f(x.x - top);
+  if (at < quads) {
+    // four cuts in flight; one without keys has left no accumulator: what is read in its place is not used
+    constexpr int U = 4;
+    const float* from = acc + row * cuts * a.d + at * 4;
+    for (int c0 = sub; c0 < cuts; c0 += U * side) {
+      f32x4 v[U];
+      float2 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = min(c0 + u * side, cuts - 1);
+        x[u] = mine[c];
+        v[u] = *reinterpret_cast<const f32x4*>(from + static_cast<long>(c) * a.d);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c0 + u * side < cuts && x[u].x > -INFINITY) o += v[u] * __builtin_amdgcn_exp2f(x[u].x - top);
     }
+  }
   for (int s = KVF_WAVE / side; s < KVF_WAVE; s *= 2)
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], s, KVF_WAVE);
@@ -396,16 +446,16 @@ __global__ __launch_bounds__(THREADS) void attn_beams_join_kernel(const float* _
   }
 }
 
-// Heads up to so many elements have room in the registers for two tiles of rows a wave.
-constexpr int TWO_TILES = 128;
-int row_tiles_of(int d, int bs, int rows) { return rows > 16 && d <= TWO_TILES && bs % 8 == 0 ? 2 : 1; }
+// Heads up to so many elements have room for two tiles of rows a wave, and for two waves a SIMD.
+template <typename T> constexpr int TWO_TILES = sizeof(T) == 2 ? 128 : 64;
+int row_tiles_of(int bf16, int d, int bs, int rows) { return rows > 16 && d <= (bf16 ? TWO_TILES<bf16_t> : TWO_TILES<float>) && bs % 8 == 0 ? 2 : 1; }
 
 template <typename T, int DT, bool ALIGNED>
 int launch_rows(const Tensors<T>& t, const Args& a, int row_tiles, hipStream_t stream) {
-  const long items = (static_cast<long>(a.n_groups) * a.cs * a.blocks + static_cast<long>(a.n_seqs) * a.co) * a.KV;
-  if (items > 0x7fffffffL) return static_cast<int>(hipErrorInvalidValue);
+  const long items = static_cast<long>(a.n_groups) * a.cs * a.blocks * a.KV + (static_cast<long>(a.n_seqs) * a.co * a.KV + WAVES - 1) / WAVES;
+  if (items * WAVES > 0x7fffffffL) return static_cast<int>(hipErrorInvalidValue);
   const dim3 grid(static_cast<unsigned>(items));
-  if constexpr (ALIGNED && DT <= TWO_TILES / 16) {
+  if constexpr (ALIGNED && DT <= TWO_TILES<T> / 16) {
     if (row_tiles == 2) {
       attn_beams_kernel<T, DT, 2, ALIGNED><<<grid, THREADS, 0, stream>>>(t, a);
       return kvf_last_error();
@@ -436,7 +486,7 @@ int run(const void* q, const void* k, const void* v, const int* table, const int
 }  // namespace
 
 // Tiles of 16 rows that a workgroup takes where a group has `rows` rows a kv head.
-KVF_EXPORT int kvf_attn_beams_row_tiles(int d, int bs, int rows) { return row_tiles_of(d, bs, rows); }
+KVF_EXPORT int kvf_attn_beams_row_tiles(int bf16, int d, int bs, int rows) { return row_tiles_of(bf16, d, bs, rows); }
 
 // q [n_seqs] rows of H heads; pages k [nb, KV, bs, d], v [nb, KV, d, bs]; table [n_seqs, width]; cu_groups [n_groups + 1];
 // shared_lens [n_groups]; ctx_lens [n_seqs].  Workspace: acc [n_seqs, H, cs + co, d], ml [n_seqs, H, cs + co, 2].
@@ -451,7 +501,7 @@ KVF_EXPORT int kvf_attn_beams(int bf16, const void* q, const void* k, const void
   if (n_seqs == 0) return 0;
   const long rows = static_cast<long>(widest) * (H / KV);
   if (rows > 1 << 20) return static_cast<int>(hipErrorInvalidValue);
-  const int row_tiles = row_tiles_of(d, bs, static_cast<int>(rows)), blocks = static_cast<int>((rows + 16 * row_tiles - 1) / (16 * row_tiles));
+  const int row_tiles = row_tiles_of(bf16, d, bs, static_cast<int>(rows)), blocks = static_cast<int>((rows + 16 * row_tiles - 1) / (16 * row_tiles));
   const Args a{H, KV, d, bs, nb, width, q_stride, o_stride, n_seqs, n_groups, blocks, cs, co, scale * LOG2E,
                bs > 1 ? static_cast<unsigned>((1ull << 32) / bs) + 1u : 0u};
   return bf16 ? run<bf16_t>(q, k, v, table, cu_groups, shared_lens, ctx_lens, out, acc, ml, sinks, a, row_tiles, stream)

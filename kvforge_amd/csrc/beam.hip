@@ -9,9 +9,9 @@
 //
 //   1. `beam_pieces_kernel`, a workgroup a piece of a row: the piece stays in registers (E logits a lane), so the row is
 //      read once.  Maximum, sum of exponentials, and the piece's `count` best, sorted.  They are found by a bound: of the
-//      64 largest logits of a wave's lanes, the `count`-th largest is settled bit by bit with ballots; at least `count`
-//      logits reach it, and seldom many more.  What reaches the best of the four waves' bounds goes to a list in LDS,
-//      where every entry counts those ahead of it: its place.  (Logits equal to the bound are taken in the order of their tokens, no
+//      64 largest logits of a wave's lanes, the `count`-th and the (count / 4)-th largest are settled bit by bit with ballots;
+//      at least `count` logits reach the best of the four waves' former and the least of their latter, and seldom many
+//      more.  What reaches the larger of the two goes to a list in LDS, where every entry counts those ahead of it: its place.  (Logits equal to the bound are taken in the order of their tokens, no
 //      more than `count` a wave, so the list holds whatever the logits are.)
 //   2. `beam_best_kernel`, a workgroup a request: joins the sums of a row's pieces in 64 bits (candidates of different
 //      beams may lie closer than 32 bits tell apart: their order is the sums' order), then merges the sorted lists of all rows,
@@ -19,32 +19,30 @@
 //      log2(count) exchanges sort them again.
 //
 // Reordering: see `beam_reorder_kernel`.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
 constexpr int THREADS = 256, NWAVES = THREADS / KVF_WAVE;
 constexpr int MAX_COUNT = 64;
+constexpr float LARGEST = 3.402823466e38f;
 
 // The order of finite numbers as unsigned integers; 0 stands below all of them ("no candidate").
 __device__ __forceinline__ uint32_t order_key(float f) {
-  const uint32_t b = __float_as_uint(f);
+  const uint32_t b = __float_as_uint(f + 0.f);       // (-0 equals 0)
   return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// exp(x) for x <= 0 to about 2^-24, without the bias that one rounded constant gives all terms of a sum: the product with
-// log2(e) is carried in two parts, the second of which joins behind the hardware's base-2 exponential.
+// exp(x) for x <= 0 (-inf too) to a few 2^-24, without the bias that a rounded log2(e) gives all terms of a sum.
 __device__ __forceinline__ float exp_unbiased(float x) {
   constexpr float L = 1.44269504088896340736f;
   constexpr float L_LO = static_cast<float>(1.44269504088896340736 - static_cast<double>(L));
-  constexpr float LN2 = 0.693147180559945f;
-  x = fmaxf(x, -200.f);            // -inf too: nothing in 32 bits
-  const float hi = x * L;
-  const float lo = fmaf(x, L, -hi) + x * L_LO;
-  const float e = __builtin_amdgcn_exp2f(hi);
-  return fmaf(e, lo * LN2, e);
+  static_assert(L_LO > 0.f, "-inf has to stay -inf");
+  return __builtin_amdgcn_exp2f(fmaf(x, L_LO, x * L));
 }
 
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -61,15 +59,15 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
   return v;
 }
 
-// The `count`-th largest of 64 lanes' keys (0 where fewer are above 0).
-__device__ __forceinline__ uint32_t kth_of_lanes(uint32_t key, int count) {
-  uint32_t found = 0;
+// The `count`-th and the `few`-th largest of 64 lanes' keys (0 where fewer are above 0).
+__device__ __forceinline__ void kth_of_lanes(uint32_t key, int count, int few, uint32_t& kth, uint32_t& high) {
+  kth = high = 0;
 #pragma unroll
   for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t want = found | (1u << bit);
-    if (__popcll(__ballot(key >= want)) >= count) found = want;
+    const uint32_t k = kth | (1u << bit), h = high | (1u << bit);
+    if (__popcll(__ballot(key >= k)) >= count) kth = k;
+    if (__popcll(__ballot(key >= h)) >= few) high = h;
   }
-  return found;
 }
 
 // 16 bytes of logits at p[0..], as keys; places outside [0, n) give 0.
@@ -86,7 +84,12 @@ template <> struct Chunk<bf16_t> {
   static __device__ __forceinline__ void load(const bf16_t* p, float (&v)[8]) { load8(p, v); }
 };
 
-__device__ __forceinline__ bool alive(float score) { return fabsf(score) <= 3.402823466e38f; }
+__device__ __forceinline__ bool alive(float score) { return fabsf(score) <= LARGEST; }
+
+// A wave's part of the list: what is strictly ahead of the bound lies in fewer than `count` of its lanes, equals are `count`
+// at most; then zeros up to a whole step.
+constexpr int LIST_STEP = 8;
+__host__ __device__ __forceinline__ int list_room(int count, int e) { return ((count - 1) * e + count + 2 * LIST_STEP - 1) / LIST_STEP * LIST_STEP; }
 
 struct PieceArgs {
   long stride;          // elements from one row of logits to the next
@@ -99,126 +102,152 @@ __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restric
                                                               double2* __restrict__ sums, float* __restrict__ values,
                                                               int* __restrict__ tokens, PieceArgs a) {
   constexpr int N = Chunk<T>::N, CHUNKS = E / N;
-  extern __shared__ unsigned long long list[];   // (key, ~token) of what reaches the bound
-  __shared__ uint32_t bound_of[NWAVES];
+  extern __shared__ __align__(16) unsigned long long list[];   // (key, ~token) of what reaches the bound, a part for every wave
+  __shared__ uint32_t bound_of[NWAVES], share_of[NWAVES];
   __shared__ float max_of[NWAVES];
   __shared__ double sum_of[NWAVES];
-  __shared__ int n_list;
+  __shared__ int n_of[NWAVES];
   const int tid = threadIdx.x, lane = tid % KVF_WAVE, wave = tid / KVF_WAVE;
   const int row = blockIdx.y, piece = blockIdx.x;
+  if (!alive(scores[row])) return;       // the whole workgroup: the merge passes such rows over
   const size_t at = static_cast<size_t>(row) * a.pieces + piece;
-  float* out_v = values + at * a.count;
-  int* out_t = tokens + at * a.count;
-  if (!alive(scores[row])) {       // the whole workgroup: the merge passes such rows over
-    return;
-  }
   const T* x = logits + row * a.stride;
   // chunks lie on 16 bytes of memory: element e of the row is place e + skip of its first chunk's line
   const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
   const int lo = piece * a.piece - skip;        // the piece's first element (below 0 in front of the row)
   const int hi = min(lo + a.piece, a.vocab);
   float v[CHUNKS][N];
+  if (lo >= 0 && lo + a.piece <= a.vocab) {
 #pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    const int e = lo + (c * THREADS + tid) * N;
-    if (e >= 0 && e + N <= hi) {
-      Chunk<T>::load(x + e, v[c]);
-    } else {
+    for (int c = 0; c < CHUNKS; ++c) Chunk<T>::load(x + lo + (c * THREADS + tid) * N, v[c]);
+  } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[c][i] = e + i >= 0 && e + i < hi ? Elem<T>::load(x + e + i) : -INFINITY;
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int e = lo + (c * THREADS + tid) * N;
+      if (e >= 0 && e + N <= hi) {
+        Chunk<T>::load(x + e, v[c]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[c][i] = e + i >= 0 && e + i < hi ? Elem<T>::load(x + e + i) : -INFINITY;
+      }
     }
   }
-  if (tid == 0) n_list = 0;
-  // NaN becomes -inf (fmaxf gives the other operand), +inf the largest finite number
-  float mx = -INFINITY;
+  // NaN becomes -inf (the maximum is the other operand), +inf the largest finite number
+  float top[CHUNKS], mx = -INFINITY;
 #pragma unroll
-  for (int c = 0; c < CHUNKS; ++c)
+  for (int c = 0; c < CHUNKS; ++c) {
+    top[c] = -INFINITY;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      v[c][i] = fminf(fmaxf(v[c][i], -INFINITY), 3.402823466e38f) + 0.f;     // (-0 equals 0)
-      mx = fmaxf(mx, v[c][i]);
+      v[c][i] = fmaxf(v[c][i], -INFINITY);
+      top[c] = fmaxf(top[c], v[c][i]);
     }
+    mx = fmaxf(mx, top[c]);
+  }
+  if (__any(mx > LARGEST)) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      top[c] = fminf(top[c], LARGEST);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[c][i] = fminf(v[c][i], LARGEST);
+    }
+    mx = fminf(mx, LARGEST);
+  }
   const uint32_t lane_key = mx > -INFINITY ? order_key(mx) : 0u;
-  const uint32_t wave_bound = kth_of_lanes(lane_key, a.count);
+  uint32_t wave_bound, wave_share;
+  kth_of_lanes(lane_key, a.count, (a.count + NWAVES - 1) / NWAVES, wave_bound, wave_share);
   const float wmx = wave_max(mx);
   if (lane == 0) {
     bound_of[wave] = wave_bound;
+    share_of[wave] = wave_share;
     max_of[wave] = wmx;
   }
   __syncthreads();
-  uint32_t bound = 0;
+  // `count` logits reach every wave's own bound, and the least of the waves' shares
+  uint32_t bound = share_of[0];
   float m = -INFINITY;
+#pragma unroll
+  for (int w = 1; w < NWAVES; ++w) bound = share_of[w] < bound ? share_of[w] : bound;
 #pragma unroll
   for (int w = 0; w < NWAVES; ++w) {
     bound = bound_of[w] > bound ? bound_of[w] : bound;
     m = fmaxf(m, max_of[w]);
   }
-  // what is ahead of the bound, and what equals it in the order of the tokens
+  // What is ahead of the bound, and what equals it in the order of the tokens.  Without a bound everything finite is taken.
   const unsigned long long below = (1ull << lane) - 1ull;
-  const float least = bound ? key_value(bound) : -INFINITY;
-  int ties = 0;
+  const float least = bound ? key_value(bound) : -LARGEST;
+  const int room = list_room(a.count, E);
+  unsigned long long* mine = list + wave * room;
+  int held = 0, ties = 0;
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < N; ++i) any |= v[c][i] >= least && v[c][i] > -INFINITY;
-    if (!__ballot(any)) continue;
+    if (!__ballot(top[c] >= least)) continue;
     const int e = lo + (c * THREADS + tid) * N;
     unsigned long long same[N];
     int before = ties, all = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const bool ahead = v[c][i] > least;
-      const unsigned long long who = __ballot(ahead);
-      if (who) {
-        int base = 0;
-        if (lane == 0) base = atomicAdd(&n_list, static_cast<int>(__popcll(who)));
-        base = __shfl(base, 0, KVF_WAVE);
-        if (ahead)
-          list[base + __popcll(who & below)] = static_cast<unsigned long long>(order_key(v[c][i])) << 32 | static_cast<uint32_t>(~(e + i));
-      }
-      same[i] = __ballot(v[c][i] == least && least > -INFINITY);
+      const unsigned long long who = __ballot(v[c][i] > least);
+      if (v[c][i] > least)
+        mine[held + __popcll(who & below)] = static_cast<unsigned long long>(order_key(v[c][i])) << 32 | static_cast<uint32_t>(~(e + i));
+      held += __popcll(who);
+      same[i] = __ballot(v[c][i] == least);
       before += __popcll(same[i] & below);
       all += __popcll(same[i]);
     }
     if (all && ties < a.count) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const bool mine = same[i] >> lane & 1ull;
-        const unsigned long long who = __ballot(mine && before < a.count);
-        if (who) {
-          int base = 0;
-          if (lane == 0) base = atomicAdd(&n_list, static_cast<int>(__popcll(who)));
-          base = __shfl(base, 0, KVF_WAVE);
-          if (mine && before < a.count)
-            list[base + __popcll(who & below)] = static_cast<unsigned long long>(bound) << 32 | static_cast<uint32_t>(~(e + i));
-        }
-        before += mine;
+        const bool equal = same[i] >> lane & 1ull;
+        const unsigned long long who = __ballot(equal && before < a.count);
+        if (equal && before < a.count)
+          mine[held + __popcll(who & below)] = static_cast<unsigned long long>(order_key(least)) << 32 | static_cast<uint32_t>(~(e + i));
+        held += __popcll(who);
+        before += equal;
       }
     }
     ties += all;
   }
-  // the sum, while the list's entries arrive
   double s = 0.0;
   if (m > -INFINITY) {
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
+    for (int c = 0; c < CHUNKS; ++c) {
+      float part = 0.f;             // of neighbours; the lane's sum is 64 bits wide
 #pragma unroll
-      for (int i = 0; i < N; ++i) s += static_cast<double>(exp_unbiased(v[c][i] - m));
-  }
-  s = wave_sum64(s);
-  if (lane == 0) sum_of[wave] = s;
-  __syncthreads();
-  const int n = n_list;
-  for (int i = tid; i < n; i += THREADS) {
-    const unsigned long long mine = list[i];
-    int place = 0;
-    for (int j = 0; j < n; ++j) place += list[j] > mine;
-    if (place < a.count) {
-      out_v[place] = key_value(static_cast<uint32_t>(mine >> 32));
-      out_t[place] = static_cast<int>(~static_cast<uint32_t>(mine));
+      for (int i = 0; i < N; ++i) part += exp_unbiased(v[c][i] - m);
+      s += static_cast<double>(part);
     }
   }
+  s = wave_sum64(s);
+  if (lane < LIST_STEP) mine[held + lane] = 0ull;       // the list is read in steps
+  if (lane == 0) {
+    sum_of[wave] = s;
+    n_of[wave] = held;
+  }
+  __syncthreads();
+  // every entry counts those ahead of it: its place
+  float* out_v = values + at * a.count;
+  int* out_t = tokens + at * a.count;
+  for (int i = lane; i < held; i += KVF_WAVE) {
+    const unsigned long long entry = mine[i];
+    int place = 0;
+#pragma unroll
+    for (int w = 0; w < NWAVES; ++w) {
+      const ulonglong2* other = reinterpret_cast<const ulonglong2*>(list + w * room);
+      for (int j = 0; j < n_of[w]; j += LIST_STEP) {
+        ulonglong2 e[LIST_STEP / 2];
+#pragma unroll
+        for (int u = 0; u < LIST_STEP / 2; ++u) e[u] = other[j / 2 + u];
+#pragma unroll
+        for (int u = 0; u < LIST_STEP / 2; ++u) place += (e[u].x > entry) + (e[u].y > entry);
+      }
+    }
+    if (place < a.count) {
+      out_v[place] = key_value(static_cast<uint32_t>(entry >> 32));
+      out_t[place] = static_cast<int>(~static_cast<uint32_t>(entry));
+    }
+  }
+  const int n = n_of[0] + n_of[1] + n_of[2] + n_of[3];
   for (int i = n + tid; i < a.count; i += THREADS) {
     out_v[i] = -INFINITY;
     out_t[i] = -1;
@@ -242,90 +271,138 @@ constexpr unsigned long long NOBODY = ~0ull;
 __device__ __forceinline__ bool ahead(const Entry& a, const Entry& b) {
   return a.score > b.score || (a.score == b.score && a.tie < b.tie);
 }
-template <typename T> __device__ __forceinline__ T from_lane(T v, int lane) { return __shfl(v, lane, KVF_WAVE); }
-__device__ __forceinline__ Entry entry_of(const Entry& e, int lane) { return {from_lane(e.score, lane), from_lane(e.tie, lane)}; }
+// The value of lane ^ O (O = 1 .. 63 of the forms below) without the LDS crossbar where it lies in the same 16 lanes: 1 and 2 are
+// permutations of four lanes, 7 and 15 the mirrors of 8 and 16, and 4 = 7 ^ 3, 8 = 15 ^ 7.
+template <int O> __device__ __forceinline__ uint32_t of_lane(uint32_t v) {
+  auto dpp = [](uint32_t x, auto ctrl) { return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, 0xF, 0xF, true)); };
+  if constexpr (O == 1) return dpp(v, std::integral_constant<int, 0xB1>{});
+  else if constexpr (O == 2) return dpp(v, std::integral_constant<int, 0x4E>{});
+  else if constexpr (O == 3) return dpp(v, std::integral_constant<int, 0x1B>{});
+  else if constexpr (O == 7) return dpp(v, std::integral_constant<int, 0x141>{});
+  else if constexpr (O == 15) return dpp(v, std::integral_constant<int, 0x140>{});
+  else if constexpr (O == 4) return of_lane<3>(of_lane<7>(v));
+  else if constexpr (O == 8) return of_lane<7>(of_lane<15>(v));
+  else return static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), O, KVF_WAVE));
+}
+template <int O> __device__ __forceinline__ unsigned long long of_lane(unsigned long long v) {
+  return static_cast<unsigned long long>(of_lane<O>(static_cast<uint32_t>(v >> 32))) << 32 | of_lane<O>(static_cast<uint32_t>(v));
+}
+template <int O> __device__ __forceinline__ Entry entry_of(const Entry& e) {
+  return {__longlong_as_double(static_cast<long long>(of_lane<O>(static_cast<unsigned long long>(__double_as_longlong(e.score))))), of_lane<O>(e.tie)};
+}
 
 // The best L of two sorted lists of L that lie in groups of L lanes (L a power of two), sorted.
+template <int O> __device__ __forceinline__ void exchange(Entry& e, int lane) {
+  if constexpr (O > 0) {
+    const Entry n = entry_of<O>(e);
+    if (((lane & O) == 0) == ahead(n, e)) e = n;
+    exchange<O / 2>(e, lane);
+  }
+}
 template <int L> __device__ __forceinline__ Entry merge_lists(Entry mine, Entry other_reversed, int lane) {
   Entry e = ahead(mine, other_reversed) ? mine : other_reversed;
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) {
-    const Entry n = entry_of(e, lane ^ o);
-    const bool first = (lane & o) == 0;
-    if (first == ahead(n, e)) e = n;
-  }
+  exchange<L / 2>(e, lane);
   return e;
+}
+// The lists of a wave's groups of L lanes, O lanes apart and more, as one in every group.
+template <int L, int O> __device__ __forceinline__ void merge_groups(Entry& e, int lane) {
+  if constexpr (O < KVF_WAVE) {
+    e = merge_lists<L>(e, entry_of<O ^ (L - 1)>(e), lane);
+    merge_groups<L, 2 * O>(e, lane);
+  }
 }
 
 struct BestArgs {
   int rows, requests, count, pieces;
 };
+constexpr int BATCH = 64;       // rows of a request that are merged at a time
 
-// row_of[row] = (reference, S - log(sum)); then the request's candidates.  L: `count` rounded up to a power of two.
-template <int L>
-__global__ __launch_bounds__(THREADS) void beam_best_kernel(const float* __restrict__ scores, const int* __restrict__ cu_beams,
-                                                            const double2* __restrict__ sums, const float* __restrict__ values,
-                                                            const int* __restrict__ tokens, double2* __restrict__ row_of,
-                                                            float* __restrict__ out_scores, int* __restrict__ out_beams,
-                                                            int* __restrict__ out_tokens, BestArgs a) {
-  __shared__ double list_s[NWAVES][L];
-  __shared__ unsigned long long list_t[NWAVES][L];
-  const int tid = threadIdx.x, lane = tid % KVF_WAVE, wave = tid / KVF_WAVE;
+// L: `count` rounded up to a power of two; W waves.
+template <int L, int W>
+__global__ __launch_bounds__(W * KVF_WAVE) void beam_best_kernel(const float* __restrict__ scores, const int* __restrict__ cu_beams,
+                                                                 const double2* __restrict__ sums, const float* __restrict__ values,
+                                                                 const int* __restrict__ tokens, float* __restrict__ out_scores,
+                                                                 int* __restrict__ out_beams, int* __restrict__ out_tokens, BestArgs a) {
+  constexpr int SIDE = KVF_WAVE / L;       // lists side by side in a wave
+  __shared__ double list_s[W][L];
+  __shared__ unsigned long long list_t[W][L];
+  __shared__ double2 row_of[BATCH];        // (reference, S - log(sum)) of a row
+  const int tid = threadIdx.x, lane = tid % KVF_WAVE, wave = tid / KVF_WAVE, group = lane / L, at = lane % L;
   const int request = blockIdx.x;
   const int first = min(max(cu_beams[request], 0), a.rows);
   const int beams = min(max(cu_beams[request + 1], first), a.rows) - first;
-  for (int b = wave; b < beams; b += NWAVES) {
-    const int row = first + b;
-    const float score = scores[row];
-    double m = -INFINITY, s = 0.0;
-    if (alive(score)) {
-      const double2* p = sums + static_cast<size_t>(row) * a.pieces;
-      for (int i = lane; i < a.pieces; i += KVF_WAVE) m = fmax(m, p[i].y);
-#pragma unroll
-      for (int o = KVF_WAVE / 2; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, KVF_WAVE));
-      if (m > -INFINITY)
-        for (int i = lane; i < a.pieces; i += KVF_WAVE) s += p[i].x * exp(p[i].y - m);
-      s = wave_sum64(s);
-    }
-    if (lane == 0) row_of[row] = make_double2(m, s > 0.0 ? static_cast<double>(score) - log(s) : -INFINITY);
-  }
-  __syncthreads();
-  const int lists = beams * a.pieces;
-  constexpr int SIDE = KVF_WAVE / L;       // lists side by side in a wave
-  const int group = lane / L, at = lane % L;
-  auto entry = [&](int l, int i) {         // entry i of list l of the request
-    Entry e{-INFINITY, NOBODY};
-    if (l < lists && i < a.count) {
-      const int beam = l / a.pieces, row = first + beam;
-      const size_t from = (static_cast<size_t>(first) * a.pieces + l) * a.count + i;
-      const double2 r = row_of[row];
-      if (r.y > -INFINITY && tokens[from] >= 0) {
-        e.score = (static_cast<double>(values[from]) - r.x) + r.y;
-        e.tie = static_cast<unsigned long long>(beam) << 48 | static_cast<unsigned long long>(~order_key(values[from])) << 16 |
-                static_cast<unsigned long long>((l - beam * a.pieces) * a.count + i);
+  Entry best{-INFINITY, NOBODY};
+  for (int b0 = 0; b0 < beams; b0 += BATCH) {
+    const int n = min(BATCH, beams - b0), lists = n * a.pieces;
+    const size_t base = static_cast<size_t>(first + b0) * a.pieces;
+    // list l of the batch, its entry i: loaded before the sums are there
+    float value;
+    int token;
+    auto load = [&](int l, int i) {
+      const bool there = l < lists && i < a.count;
+      const size_t from = (base + (there ? l : 0)) * a.count + (there ? i : 0);
+      value = values[from];
+      token = there ? tokens[from] : -1;
+    };
+    auto entry = [&](int l, int i) {
+      Entry e{-INFINITY, NOBODY};
+      if (token >= 0) {
+        const int beam = l / a.pieces;
+        const double2 r = row_of[beam];
+        if (r.y > -INFINITY) {
+          e.score = (static_cast<double>(value) - r.x) + r.y;
+          e.tie = static_cast<unsigned long long>(b0 + beam) << 48 | static_cast<unsigned long long>(~order_key(value)) << 16 |
+                  static_cast<unsigned long long>((l - beam * a.pieces) * a.count + i);
+        }
       }
-    }
-    return e;
-  };
-  int l = wave * SIDE + group;
-  Entry best = entry(l, at);
-  for (l += NWAVES * SIDE; l - group < lists; l += NWAVES * SIDE) best = merge_lists<L>(best, entry(l, L - 1 - at), lane);
+      return e;
+    };
+    // `best` is sorted, so the other list is taken from its end
+    int l = wave * SIDE + group;
+    load(l, L - 1 - at);
+    if (b0) __syncthreads();
+    for (int b = wave; b < n; b += W) {
+      const int row = first + b0 + b;
+      const float score = scores[row];
+      double m = -INFINITY, s = 0.0;
+      if (alive(score)) {
+        const double2* p = sums + static_cast<size_t>(row) * a.pieces;
+        double2 mine = lane < a.pieces ? p[lane] : make_double2(0.0, -INFINITY);
+        m = mine.y;
+        for (int i = lane + KVF_WAVE; i < a.pieces; i += KVF_WAVE) m = fmax(m, p[i].y);
 #pragma unroll
-  for (int o = L; o < KVF_WAVE; o <<= 1) {      // the groups of the wave
-    const Entry other = entry_of(best, (lane ^ o) ^ (L - 1));
-    best = merge_lists<L>(best, other, lane);
+        for (int o = KVF_WAVE / 2; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, KVF_WAVE));
+        if (m > -INFINITY) {
+          s = mine.x * exp(mine.y - m);
+          for (int i = lane + KVF_WAVE; i < a.pieces; i += KVF_WAVE) s += p[i].x * exp(p[i].y - m);
+        }
+        s = wave_sum64(s);
+      }
+      if (lane == 0) row_of[b] = make_double2(m, s > 0.0 ? static_cast<double>(score) - log(s) : -INFINITY);
+    }
+    __syncthreads();
+    while (l - group < lists) {
+      const Entry e = entry(l, L - 1 - at);
+      l += W * SIDE;
+      if (l - group < lists) load(l, L - 1 - at);
+      best = merge_lists<L>(best, e, lane);
+    }
   }
+  merge_groups<L, L>(best, lane);
   if (lane < L) {
     list_s[wave][lane] = best.score;
     list_t[wave][lane] = best.tie;
   }
   __syncthreads();
   if (wave > 0) return;
-#pragma unroll
-  for (int w = 1; w < NWAVES; ++w) {
-    const Entry other{list_s[w][L - 1 - at], list_t[w][L - 1 - at]};
+  // the waves' lists, those that the groups hold already left out: group g takes g, g + SIDE, ...
+  best = group < W ? Entry{list_s[group][at], list_t[group][at]} : Entry{-INFINITY, NOBODY};
+  for (int w = SIDE; w < W; w += SIDE) {
+    const int take = w + group;
+    const Entry other = take < W ? Entry{list_s[take][L - 1 - at], list_t[take][L - 1 - at]} : Entry{-INFINITY, NOBODY};
     best = merge_lists<L>(best, other, lane);
   }
+  merge_groups<L, L>(best, lane);
   if (lane < a.count) {
     const bool there = best.tie != NOBODY;
     const int beam = static_cast<int>(best.tie >> 48);
@@ -338,19 +415,17 @@ __global__ __launch_bounds__(THREADS) void beam_best_kernel(const float* __restr
 
 template <typename T, int E>
 int pieces_launch(const void* logits, const float* scores, double2* sums, float* values, int* tokens, const PieceArgs& a, hipStream_t stream) {
-  // what is strictly ahead of the bound lies in fewer than `count` lanes of every wave; equals: `count` a wave
-  const size_t lds = static_cast<size_t>(NWAVES) * ((a.count - 1) * E + a.count) * sizeof(unsigned long long);
+  const size_t lds = static_cast<size_t>(NWAVES) * list_room(a.count, E) * sizeof(unsigned long long);
   beam_pieces_kernel<T, E><<<dim3(a.pieces, a.rows), THREADS, lds, stream>>>(static_cast<const T*>(logits), scores, sums, values, tokens, a);
   return kvf_last_error();
 }
 }  // namespace
 
 // logits [rows][stride] of `vocab` (bf16: 0 fp32, 1 bf16); scores [rows]; cu_beams [requests + 1]; out_* [requests][count].
-// Workspace: sums [rows][pieces][2] and row_of [rows][2] in 64 bits, values/tokens [rows][pieces][count].  piece: elements of a
+// Workspace: sums [rows][pieces][2] in 64 bits, values/tokens [rows][pieces][count].  piece: elements of a
 // piece, 256 times 8 or 32.
 KVF_EXPORT int kvf_beam_select(int bf16, const void* logits, long stride, int rows, int vocab, const float* scores,
-                               const int* cu_beams, int requests, int count, int pieces, int piece, void* sums, void* row_of,
-                               float* values, int* tokens, float* out_scores, int* out_beams, int* out_tokens,
+                               const int* cu_beams, int requests, int count, int pieces, int piece, void* sums, float* values, int* tokens, float* out_scores, int* out_beams, int* out_tokens,
                                hipStream_t stream) {
   if (count < 1 || count > MAX_COUNT || rows < 0 || rows > 65535 || vocab < 1 || pieces < 1 || requests < 0 ||
       static_cast<long>(pieces) * count > 65536)
@@ -373,8 +448,13 @@ KVF_EXPORT int kvf_beam_select(int bf16, const void* logits, long stride, int ro
   }
   const BestArgs b{rows, requests, count, pieces};
   const auto* s = static_cast<const double2*>(sums);
-  auto* r = static_cast<double2*>(row_of);
-#define KVF_BEST(L) beam_best_kernel<L><<<requests, THREADS, 0, stream>>>(scores, cu_beams, s, values, tokens, r, out_scores, out_beams, out_tokens, b)
+  // more waves where a request has lists for them on average
+  const bool wide = static_cast<long>(rows) * pieces > 16L * requests;
+#define KVF_BEST(L)                                                                                                                       \
+  do {                                                                                                                                    \
+    if (wide) beam_best_kernel<L, 16><<<requests, 16 * KVF_WAVE, 0, stream>>>(scores, cu_beams, s, values, tokens, out_scores, out_beams, out_tokens, b); \
+    else beam_best_kernel<L, 4><<<requests, 4 * KVF_WAVE, 0, stream>>>(scores, cu_beams, s, values, tokens, out_scores, out_beams, out_tokens, b);        \
+  } while (0)
   if (count <= 4) KVF_BEST(4);
   else if (count <= 8) KVF_BEST(8);
   else if (count <= 16) KVF_BEST(16);
@@ -385,85 +465,129 @@ KVF_EXPORT int kvf_beam_select(int bf16, const void* logits, long stride, int ro
 }
 
 namespace {
-// What a set of tensors is made of: tensor t has rows of `bytes` bytes, `stride` bytes apart, read and written `unit` bytes at a time.
-struct RowsOf {
-  char* base;
-  long stride, bytes, unit;
-};
-struct Tile {
-  int tensor, number;    // tile `number` of the tensor's rows: TILE_BYTES of them
-};
 constexpr int TILE_BYTES = THREADS * 16;
+// Up to TILE_BYTES bytes of a tensor's row 0 from `base` on; rows are `stride` bytes apart and moved `unit` bytes at a time.
+struct Tile {
+  char* base;
+  long stride;
+  int bytes, unit;
+};
 
-template <typename U> struct Words { static constexpr int N = 16 / sizeof(U); };
-
-// A workgroup takes a tile of bytes of one tensor, of all W rows of a request: a lane's bytes of every row that moves are in its
-// registers before it writes any of them, and no other lane touches them, so rows may change places in any way (swaps and rings
-// too) without memory beside them.
-template <typename U, int W>
-__device__ __forceinline__ void move_rows(const RowsOf& t, int number, int rows, int beams, const int* __restrict__ slots,
-                                          const int* __restrict__ parents) {
-  constexpr int N = Words<U>::N;
-  U v[W][N];
-  const long from = static_cast<long>(number) * TILE_BYTES + threadIdx.x * sizeof(U);
-  int to[W];
+// Where the rows of a request's beams come from and go to; row -1: nothing moves.  A lane a beam, so that two loads find out
+// about all of them.
+template <int W> struct Moves {
+  int from[W], to[W];
+  __device__ __forceinline__ void read(const int* __restrict__ slots, const int* __restrict__ parents, int beams, int rows) {
+    const int lane = threadIdx.x % KVF_WAVE;
+    const int p = lane < beams ? parents[lane] : -1, dst = lane < beams ? slots[lane] : -1;
+    const bool named = p != lane && p >= 0 && p < beams;
+    const int src = __shfl(dst, named ? p : lane, KVF_WAVE);
+    const bool moves = named && dst >= 0 && dst < rows && src >= 0 && src < rows && src != dst;
 #pragma unroll
-  for (int b = 0; b < W; ++b) {
-    to[b] = -1;
-    if (b >= beams) continue;
-    const int p = parents[b];
-    if (p == b || p < 0 || p >= beams) continue;
-    const int dst = slots[b], src = slots[p];
-    if (dst < 0 || dst >= rows || src < 0 || src >= rows || src == dst) continue;
-    to[b] = dst;
-    const char* row = t.base + src * t.stride;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const long o = from + static_cast<long>(i) * THREADS * sizeof(U);
-      if (o < t.bytes) v[b][i] = *reinterpret_cast<const U*>(row + o);
+    for (int b = 0; b < W; ++b) {
+      from[b] = __builtin_amdgcn_readlane(moves ? src : -1, b);
+      to[b] = __builtin_amdgcn_readlane(moves ? dst : -1, b);
     }
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // all read before any is written
+};
+
+// Bytes of device memory, by the type that they are moved as: vectors of the language (arrays of HIP's own go through LDS) behind
+// pointers known to be global (one read from a table may point anywhere, and its loads wait on the LDS counter too).
+typedef uint32_t Word4 __attribute__((ext_vector_type(4)));
+typedef uint32_t Word2 __attribute__((ext_vector_type(2)));
+template <typename Unit> __device__ __forceinline__ Unit get(const char* base, long at) {
+  return *(const __attribute__((address_space(1))) Unit*)(base + at);
+}
+template <typename Unit> __device__ __forceinline__ void put(char* base, long at, Unit v) {
+  *(__attribute__((address_space(1))) Unit*)(base + at) = v;
+}
+
+// All loads have arrived, and the compiler knows it: otherwise it waits again ahead of every store, and with it for the stores
+// before (eight requests of four beams, 1 MB rows of eight tensors: 101 us, and 44 so).
+__device__ __forceinline__ void loads_arrived() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);      // vmcnt 0, the other counters as they are
+  asm volatile("" ::: "memory");
+}
+
+// A tile of all rows of a request: a lane's bytes of every row that moves are in its registers before it writes any of them, and
+// no other lane touches them, so rows may change places in any way (swaps and rings too) without memory beside them.
+// U whole tiles, 16 bytes at a time:
+template <int W, int U> __device__ __forceinline__ void move_whole(const Tile (&t)[U], const Moves<W>& m) {
+  Word4 v[W][U];
+  const int at = threadIdx.x * 16;
 #pragma unroll
-  for (int b = 0; b < W; ++b) {
-    if (to[b] < 0) continue;
-    char* row = t.base + to[b] * t.stride;
+  for (int b = 0; b < W; ++b)
+    if (m.to[b] >= 0)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const long o = from + static_cast<long>(i) * THREADS * sizeof(U);
-      if (o < t.bytes) *reinterpret_cast<U*>(row + o) = v[b][i];
-    }
+      for (int u = 0; u < U; ++u) v[b][u] = get<Word4>(t[u].base + m.from[b] * t[u].stride, at);
+  loads_arrived();
+#pragma unroll
+  for (int b = 0; b < W; ++b)
+    if (m.to[b] >= 0)
+#pragma unroll
+      for (int u = 0; u < U; ++u) put(t[u].base + m.to[b] * t[u].stride, at, v[b][u]);
+}
+// any tile:
+template <typename Unit, int W> __device__ __forceinline__ void move_any(const Tile& t, const Moves<W>& m) {
+  constexpr int SIZE = sizeof(Unit);
+  for (int at = threadIdx.x * SIZE; at < t.bytes; at += THREADS * SIZE) {
+    Unit v[W];
+#pragma unroll
+    for (int b = 0; b < W; ++b)
+      if (m.to[b] >= 0) v[b] = get<Unit>(t.base + m.from[b] * t.stride, at);
+    loads_arrived();
+#pragma unroll
+    for (int b = 0; b < W; ++b)
+      if (m.to[b] >= 0) put(t.base + m.to[b] * t.stride, at, v[b]);
   }
 }
 
-template <int W>
-__global__ __launch_bounds__(THREADS) void beam_reorder_kernel(const RowsOf* __restrict__ tensors, const Tile* __restrict__ tiles,
-                                                               int rows, int beams, const int* __restrict__ slots,
-                                                               const int* __restrict__ parents) {
-  const Tile tile = tiles[blockIdx.x];
-  const RowsOf t = tensors[tile.tensor];
-  slots += static_cast<size_t>(blockIdx.y) * beams;
-  parents += static_cast<size_t>(blockIdx.y) * beams;
-  if (t.unit == 16) move_rows<uint4, W>(t, tile.number, rows, beams, slots, parents);
-  else if (t.unit == 8) move_rows<uint2, W>(t, tile.number, rows, beams, slots, parents);
-  else if (t.unit == 4) move_rows<uint32_t, W>(t, tile.number, rows, beams, slots, parents);
-  else move_rows<uint16_t, W>(t, tile.number, rows, beams, slots, parents);
+template <int W, int U>
+__global__ __launch_bounds__(THREADS) void beam_reorder_kernel(const Tile* __restrict__ tiles, int n_tiles, int rows, int beams,
+                                                               const int* __restrict__ slots, const int* __restrict__ parents) {
+  Tile t[U];
+  bool whole = true;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = blockIdx.x * U + u;
+    t[u] = tiles[min(i, n_tiles - 1)];
+    whole &= i < n_tiles && t[u].unit == 16 && t[u].bytes == TILE_BYTES;
+  }
+  Moves<W> m;
+  m.read(slots + static_cast<size_t>(blockIdx.y) * beams, parents + static_cast<size_t>(blockIdx.y) * beams, beams, rows);
+  if (whole) {
+    move_whole<W, U>(t, m);
+    return;
+  }
+#pragma unroll 1
+  for (int i = blockIdx.x * U; i < min(static_cast<int>(blockIdx.x) * U + U, n_tiles); ++i) {
+    const Tile one = tiles[i];
+    if (one.unit == 16) move_any<Word4, W>(one, m);
+    else if (one.unit == 8) move_any<Word2, W>(one, m);
+    else if (one.unit == 4) move_any<uint32_t, W>(one, m);
+    else move_any<uint16_t, W>(one, m);
+  }
+}
+
+template <int W, int U>
+void reorder_launch(const Tile* tiles, int n_tiles, int rows, int requests, int beams, const int* slots, const int* parents, hipStream_t stream) {
+  beam_reorder_kernel<W, U><<<dim3((n_tiles + U - 1) / U, requests), THREADS, 0, stream>>>(tiles, n_tiles, rows, beams, slots, parents);
 }
 }  // namespace
 
 KVF_EXPORT int kvf_beam_tile_bytes() { return TILE_BYTES; }
 
-// tensors: RowsOf (four 64-bit numbers) each; tiles: (tensor, number) each; slots, parents [requests][beams].
-KVF_EXPORT int kvf_beam_reorder(const void* tensors, const void* tiles, int n_tiles, int rows, int requests, int beams,
-                                const int* slots, const int* parents, hipStream_t stream) {
+// tiles: Tile (address, bytes from row to row, bytes of the tile | unit << 32: three 64-bit numbers) each; slots, parents
+// [requests][beams].
+KVF_EXPORT int kvf_beam_reorder(const void* tiles, int n_tiles, int rows, int requests, int beams, const int* slots, const int* parents,
+                                hipStream_t stream) {
+  static_assert(sizeof(Tile) == 24, "as the table is written");
   if (beams < 1 || beams > 32 || requests < 0 || requests > 65535 || n_tiles < 0 || rows < 0) return static_cast<int>(hipErrorInvalidValue);
   if (requests == 0 || n_tiles == 0 || beams == 1) return 0;
-  const auto* t = static_cast<const RowsOf*>(tensors);
-  const auto* l = static_cast<const Tile*>(tiles);
-  const dim3 grid(n_tiles, requests);
-  if (beams <= 4) beam_reorder_kernel<4><<<grid, THREADS, 0, stream>>>(t, l, rows, beams, slots, parents);
-  else if (beams <= 8) beam_reorder_kernel<8><<<grid, THREADS, 0, stream>>>(t, l, rows, beams, slots, parents);
-  else if (beams <= 16) beam_reorder_kernel<16><<<grid, THREADS, 0, stream>>>(t, l, rows, beams, slots, parents);
-  else beam_reorder_kernel<32><<<grid, THREADS, 0, stream>>>(t, l, rows, beams, slots, parents);
+  const auto* t = static_cast<const Tile*>(tiles);
+  if (beams <= 4) reorder_launch<4, 4>(t, n_tiles, rows, requests, beams, slots, parents, stream);
+  else if (beams <= 8) reorder_launch<8, 2>(t, n_tiles, rows, requests, beams, slots, parents, stream);
+  else if (beams <= 16) reorder_launch<16, 2>(t, n_tiles, rows, requests, beams, slots, parents, stream);
+  else reorder_launch<32, 1>(t, n_tiles, rows, requests, beams, slots, parents, stream);
   return kvf_last_error();
 }

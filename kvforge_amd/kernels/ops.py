@@ -1725,12 +1725,22 @@ ATTN_BEAMS_KEYS_PER_CUT = 256
 
 def _here(who: str, first: torch.Tensor, *others) -> None:
     """Launches go to the current device's stream: every operand lives there."""
-    at = first.device
-    if at.index != torch.cuda.current_device():
-        raise KernelError(f"{who}: operands live on {at}, the current device is {torch.cuda.current_device()}")
+    at = first.get_device()
+    if at != torch.cuda.current_device():
+        raise KernelError(f"{who}: operands live on device {at}, the current one is {torch.cuda.current_device()}")
     for t in others:
-        if t is not None and t.device != at:
+        if t is not None and t.get_device() != at:
             raise KernelError(f"{who}: operands live on several devices")
+
+
+def _apart(outs, ins) -> bool:
+    """Whether the memory of dense tensors ``outs`` lies apart from that of ``ins``, given as (address, bytes)."""
+    for o in outs:
+        a, b = o.data_ptr(), o.nbytes
+        for c, n in ins:
+            if a < c + n and c < a + b:
+                return False
+    return True
 
 
 def attn_beams_takes(dtype: torch.dtype, head_dim: int) -> bool:
@@ -1741,17 +1751,19 @@ def attn_beams_takes(dtype: torch.dtype, head_dim: int) -> bool:
 def attn_beams_cuts(q: torch.Tensor, k_pages: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, num_groups: int,
                     num_seqs: int, widest: int, max_shared: int, max_own: int) -> tuple[int, int]:
     """(cuts of the keys that a group shares, cuts of a sequence's own keys) for ``attn_beams``: two workgroups a compute unit
-    where the keys suffice for cuts of ``ATTN_BEAMS_KEYS_PER_CUT``.  ``max_shared``, ``max_own``: the most shared keys of a
-    group and own keys of a sequence (any cuts give right results for any lengths)."""
-    room = 2 * compute_units(q.device)
+    over the shared keys and 16 waves over the others, where the keys suffice for cuts of ``ATTN_BEAMS_KEYS_PER_CUT`` and a quarter
+    of it.  ``max_shared``, ``max_own``: the most shared keys of a group and own keys of a sequence (any cuts give right
+    results for any lengths)."""
+    units = compute_units(q.device)
     rows = max(1, widest) * (num_heads // num_kv_heads)
-    tiles = int(_fn("attn_beams", "kvf_attn_beams_row_tiles", [c_int] * 3)(head_dim, k_pages.shape[2], rows))
+    tiles = int(_fn("attn_beams", "kvf_attn_beams_row_tiles", [c_int] * 4)(_tcode(q.dtype), head_dim, k_pages.shape[2], rows))
     shared = num_groups * num_kv_heads * -(-rows // (16 * tiles))
 
-    def cuts(groups: int, keys: int) -> int:
-        return max(1, min(-(-room // max(groups, 1)), -(-keys // ATTN_BEAMS_KEYS_PER_CUT), ATTN_BEAMS_MAX_CUTS))
+    def cuts(room: int, groups: int, keys: int, per: int) -> int:
+        return max(1, min(-(-room // max(groups, 1)), -(-keys // per), ATTN_BEAMS_MAX_CUTS))
 
-    return (cuts(shared, max_shared) if num_groups and max_shared > 0 else 0), cuts(num_seqs * num_kv_heads, max_own)
+    return (cuts(2 * units, shared, max_shared, ATTN_BEAMS_KEYS_PER_CUT) if num_groups and max_shared > 0 else 0,
+            cuts(16 * units, num_seqs * num_kv_heads, max_own, ATTN_BEAMS_KEYS_PER_CUT // 4))
 
 
 def attn_beams_workspace(num_seqs: int, num_heads: int, head_dim: int, cuts: tuple[int, int], device
@@ -1800,7 +1812,7 @@ def attn_beams(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     _check(shared_lens, "shared_lens", I32, (groups,))
     _check(ctx_lens, "ctx_lens", I32, (n,))
     _check(out, "out", q.dtype, (n, H * d))
-    if out.data_ptr() % 16 or _overlap(out, q):
+    if out.data_ptr() % 16 or (n and not _apart((out,), ((q.data_ptr(), ((n - 1) * q.stride(0) + H * d) * size),))):
         raise KernelError("attn_beams: out starts on 16 bytes and does not share memory with q")
     cs, co = int(cuts[0]), int(cuts[1])
     if not (0 <= cs <= ATTN_BEAMS_MAX_CUTS and 1 <= co <= ATTN_BEAMS_MAX_CUTS):
@@ -2894,11 +2906,10 @@ def _beam_pieces(rows: int, vocab: int, count: int, device) -> tuple[int, int]:
 
 
 def beam_select_workspace(rows: int, vocab: int, count: int, device) -> tuple[torch.Tensor, ...]:
-    """Scratch of ``beam_select`` for ``rows`` rows of logits: the pieces' sums and the rows', the pieces' best logits and
-    their tokens."""
+    """Scratch of ``beam_select`` for ``rows`` rows of logits: the pieces' sums, their best logits and the tokens of
+    these."""
     pieces, _ = _beam_pieces(rows, vocab, count, device)
     return (torch.empty(rows * pieces * 2, dtype=torch.float64, device=device),
-            torch.empty(rows * 2, dtype=torch.float64, device=device),
             torch.empty(rows * pieces * count, dtype=F32, device=device),
             torch.empty(rows * pieces * count, dtype=I32, device=device))
 
@@ -2930,37 +2941,38 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, cu_beams: torch.Tens
         raise KernelError(f"beam_select gives 1 to {BEAM_MAX_COUNT} candidates a request, asked for {count}")
     _check(out_beams, "out_beams", I32, (requests, count))
     _check(out_tokens, "out_tokens", I32, (requests, count))
-    if any(_overlap(o, i) for o in (out_scores, out_beams, out_tokens) for i in (scores, logits, cu_beams)):
+    stride = logits.stride(0) if rows > 1 else vocab
+    if rows and not _apart((out_scores, out_beams, out_tokens),
+                           ((logits.data_ptr(), ((rows - 1) * stride + vocab) * logits.element_size()),
+                            (scores.data_ptr(), 4 * rows), (cu_beams.data_ptr(), 4 * requests + 4))):
         raise KernelError("beam_select: outputs do not share memory with inputs")
     pieces, piece = _beam_pieces(rows, vocab, count, logits.device)
     if pieces * count > 65536 or rows * pieces * count >= 2**31:
         raise KernelError(f"beam_select: {count} candidates of each of {pieces} pieces of {rows} rows are more than the kernel counts")
-    sums, row_of, values, tokens = workspace
+    sums, values, tokens = workspace
     _check(sums, "workspace[0]", torch.float64, (None,))
-    _check(row_of, "workspace[1]", torch.float64, (None,))
-    _check(values, "workspace[2]", F32, (None,))
-    _check(tokens, "workspace[3]", I32, (None,))
-    if (sums.shape[0] < rows * pieces * 2 or row_of.shape[0] < rows * 2
-            or min(values.shape[0], tokens.shape[0]) < rows * pieces * count or sums.data_ptr() % 16 or row_of.data_ptr() % 16):
+    _check(values, "workspace[1]", F32, (None,))
+    _check(tokens, "workspace[2]", I32, (None,))
+    if (sums.shape[0] < rows * pieces * 2 or min(values.shape[0], tokens.shape[0]) < rows * pieces * count or sums.data_ptr() % 16):
         raise KernelError("beam_select: workspace too small for these rows, logits and candidates")
     _here("beam_select", logits, scores, cu_beams, out_scores, out_beams, out_tokens, *workspace)
-    f = _fn("beam", "kvf_beam_select", [c_int, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 8)
-    _ok(f(_tcode(logits.dtype), logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, scores.data_ptr(),
-          cu_beams.data_ptr(), requests, count, pieces, piece, sums.data_ptr(), row_of.data_ptr(), values.data_ptr(),
+    f = _fn("beam", "kvf_beam_select", [c_int, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 7)
+    _ok(f(_tcode(logits.dtype), logits.data_ptr(), stride, rows, vocab, scores.data_ptr(),
+          cu_beams.data_ptr(), requests, count, pieces, piece, sums.data_ptr(), values.data_ptr(),
           tokens.data_ptr(), out_scores.data_ptr(), out_beams.data_ptr(), out_tokens.data_ptr(), _stream()), "beam_select")
 
 
 class CacheRows:
     """Tensors whose rows (pages, or state slots, of every layer) move together: ``beam_reorder`` moves the same rows in all
-    of them with one launch.  Rows are dense; they may be columns of wider ones.  Keeps the tensors, and a table of them on
-    their device."""
+    of them with one launch.  Rows are dense; they may be columns of wider ones.  Keeps the tensors, and a table of the pieces
+    of their rows on their device."""
 
     def __init__(self, tensors) -> None:
         self.tensors = list(tensors)
         if not self.tensors:
             raise KernelError("CacheRows: at least one tensor")
         first = self.tensors[0]
-        spans, table, tiles = [], [], []
+        spans, tiles = [], []
         tile_bytes = int(_fn("beam", "kvf_beam_tile_bytes", [])())
         for t in self.tensors:
             _check(t, "tensor", None, None, contiguous=False)
@@ -2978,12 +2990,11 @@ class CacheRows:
                     raise KernelError("CacheRows: rows of different tensors share memory")
             spans.append((at, stride, row))
             unit = next(u for u in (16, 8, 4, 2) if at % u == 0 and stride % u == 0 and row % u == 0)
-            table.append((at, stride, row, unit))
-            tiles.append(-(-row // tile_bytes))
+            from_ = torch.arange(0, row, tile_bytes, dtype=torch.int64)
+            tiles.append(torch.stack([from_ + at, torch.full_like(from_, stride),
+                                      (row - from_).clamp(max=tile_bytes) + (unit << 32)], dim=1))
         self.rows, self.device = int(first.shape[0]), first.device
-        self.table = torch.tensor(table, dtype=torch.int64, device=self.device)
-        self.tiles = torch.cat([torch.stack([torch.full((n,), i, dtype=I32), torch.arange(n, dtype=I32)], dim=1)
-                                for i, n in enumerate(tiles)]).contiguous().to(self.device)
+        self.tiles = torch.cat(tiles).to(self.device)
 
 
 def beam_reorder(rows: CacheRows, slots: torch.Tensor, parents: torch.Tensor) -> None:
@@ -2996,7 +3007,7 @@ def beam_reorder(rows: CacheRows, slots: torch.Tensor, parents: torch.Tensor) ->
     _check(parents, "parents", I32, (requests, beams))
     if not 1 <= beams <= BEAM_MAX_WIDTH or requests > 65535:
         raise KernelError(f"beam_reorder takes up to 65535 requests of 1 to {BEAM_MAX_WIDTH} beams, got {requests} of {beams}")
-    _here("beam_reorder", rows.table, slots, parents)
-    f = _fn("beam", "kvf_beam_reorder", [c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 3)
-    _ok(f(rows.table.data_ptr(), rows.tiles.data_ptr(), rows.tiles.shape[0], rows.rows, requests, beams, slots.data_ptr(),
+    _here("beam_reorder", rows.tiles, slots, parents)
+    f = _fn("beam", "kvf_beam_reorder", [c_void_p] + [c_int] * 4 + [c_void_p] * 3)
+    _ok(f(rows.tiles.data_ptr(), rows.tiles.shape[0], rows.rows, requests, beams, slots.data_ptr(),
           parents.data_ptr(), _stream()), "beam_reorder")

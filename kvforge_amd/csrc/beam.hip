@@ -7,16 +7,20 @@
 // Logits that are NaN or -inf are no candidates and weigh nothing, +inf counts as the largest finite number, and
 // beams whose score is not finite are passed over unread.
 //
-//   1. `beam_pieces_kernel`, a workgroup a piece of a row: the piece stays in registers (E logits a lane), so the row is
-//      read once.  Maximum, sum of exponentials, and the piece's `count` best, sorted.  They are found by a bound: of the
-//      64 largest logits of a wave's lanes, the `count`-th and the (count / 4)-th largest are settled bit by bit with ballots;
-//      at least `count` logits reach the best of the four waves' former and the least of their latter, and seldom many
-//      more.  What reaches the larger of the two goes to a list in LDS, where every entry counts those ahead of it: its place.  (Logits equal to the bound are taken in the order of their tokens, no
-//      more than `count` a wave, so the list holds whatever the logits are.)
-//   2. `beam_best_kernel`, a workgroup a request: joins the sums of a row's pieces in 64 bits (candidates of different
-//      beams may lie closer than 32 bits tell apart: their order is the sums' order), then merges the sorted lists of all rows,
-//      the lists of a wave side by side: of two sorted lists the larger of a[i] and b[count - 1 - i] are the best of both, and
-//      log2(count) exchanges sort them again.
+//   1. `beam_pieces_kernel`: a workgroup takes a piece of a row, which stays in its registers (E logits a lane), so the row is read once.  Maximum, sum of
+//      exponentials, and the piece's `count` best, sorted.  They are found by a bound: of the 64 largest logits of a wave's
+//      lanes, the `count`-th and the (count / 4)-th largest are settled bit by bit with ballots; at least `count` logits reach
+//      the best of the four waves' former and the least of their latter, and seldom many more.  What reaches the larger of the
+//      two goes to a list in LDS, where every entry counts those ahead of it: its place.  (Logits equal to the bound are taken
+//      in the order of their tokens, no more than `count` a wave, so the list holds whatever the logits are.)
+//   2. `beam_best_kernel`: a workgroup a request joins the sums of a row's pieces in 64 bits (candidates of different
+//      beams may lie closer than 32 bits tell apart: their order is the sums' order), then picks among the pieces' best by a
+//      bound and by counting again.  Where equal scores let too many entries reach the bound, the sorted lists are merged
+//      instead, those of a wave side by side: of two sorted lists the larger of a[i] and b[count - 1 - i] are the best of both,
+//      and log2(count) exchanges sort them again.
+//   (One kernel, in which the workgroup of a request that is done last goes on with 2, saves 3 us of the host's time but takes
+//   longer on the device, since results have to pass the XCDs' L2s and 2's registers are 1's too: 4 rows of 8,192 logits 13.4 us
+//   and 10.3 so, 32 rows of 128,256 18.0 and 13.6, 512 rows 79 and 62.)
 //
 // Reordering: see `beam_reorder_kernel`.
 #include <type_traits>
@@ -45,25 +49,48 @@ __device__ __forceinline__ float exp_unbiased(float x) {
   return __builtin_amdgcn_exp2f(fmaf(x, L_LO, x * L));
 }
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int o = KVF_WAVE / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, KVF_WAVE);
-  return v;
+// The value of lane ^ O (O = 1 .. 63 of the forms below) without the LDS crossbar where it lies in the same 16 lanes: 1 and 2 are
+// permutations of four lanes, 7 and 15 the mirrors of 8 and 16, and 4 = 7 ^ 3, 8 = 15 ^ 7.
+template <int O> __device__ __forceinline__ uint32_t of_lane(uint32_t v) {
+  auto dpp = [](uint32_t x, auto ctrl) { return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, 0xF, 0xF, true)); };
+  if constexpr (O == 1) return dpp(v, std::integral_constant<int, 0xB1>{});
+  else if constexpr (O == 2) return dpp(v, std::integral_constant<int, 0x4E>{});
+  else if constexpr (O == 3) return dpp(v, std::integral_constant<int, 0x1B>{});
+  else if constexpr (O == 7) return dpp(v, std::integral_constant<int, 0x141>{});
+  else if constexpr (O == 15) return dpp(v, std::integral_constant<int, 0x140>{});
+  else if constexpr (O == 4) return of_lane<3>(of_lane<7>(v));
+  else if constexpr (O == 8) return of_lane<7>(of_lane<15>(v));
+  else return static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), O, KVF_WAVE));
 }
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-  for (int o = KVF_WAVE / 2; o > 0; o >>= 1) {
-    const uint32_t n = __shfl_xor(v, o, KVF_WAVE);
-    v = n > v ? n : v;
-  }
-  return v;
+template <int O> __device__ __forceinline__ unsigned long long of_lane(unsigned long long v) {
+  return static_cast<unsigned long long>(of_lane<O>(static_cast<uint32_t>(v >> 32))) << 32 | of_lane<O>(static_cast<uint32_t>(v));
+}
+template <int O> __device__ __forceinline__ double of_lane(double v) {
+  return __longlong_as_double(static_cast<long long>(of_lane<O>(static_cast<unsigned long long>(__double_as_longlong(v)))));
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+  v += of_lane<1>(v);
+  v += of_lane<2>(v);
+  v += of_lane<7>(v);       // the other four of 8 lanes
+  v += of_lane<15>(v);      // the other eight of 16
+  v += of_lane<16>(v);
+  return v + of_lane<32>(v);
+}
+__device__ __forceinline__ float wave_most(float v) {
+  auto of = [](float x, auto o) { return __uint_as_float(of_lane<decltype(o)::value>(__float_as_uint(x))); };
+  v = fmaxf(v, of(v, std::integral_constant<int, 1>{}));
+  v = fmaxf(v, of(v, std::integral_constant<int, 2>{}));
+  v = fmaxf(v, of(v, std::integral_constant<int, 7>{}));
+  v = fmaxf(v, of(v, std::integral_constant<int, 15>{}));
+  v = fmaxf(v, of(v, std::integral_constant<int, 16>{}));
+  return fmaxf(v, of(v, std::integral_constant<int, 32>{}));
 }
 
-// The `count`-th and the `few`-th largest of 64 lanes' keys (0 where fewer are above 0).
-__device__ __forceinline__ void kth_of_lanes(uint32_t key, int count, int few, uint32_t& kth, uint32_t& high) {
+// The `count`-th and the `few`-th largest of 64 lanes' keys (0 where fewer are above 0), down to bit LOW.
+template <int LOW> __device__ __forceinline__ void kth_of_lanes(uint32_t key, int count, int few, uint32_t& kth, uint32_t& high) {
   kth = high = 0;
 #pragma unroll
-  for (int bit = 31; bit >= 0; --bit) {
+  for (int bit = 31; bit >= LOW; --bit) {
     const uint32_t k = kth | (1u << bit), h = high | (1u << bit);
     if (__popcll(__ballot(key >= k)) >= count) kth = k;
     if (__popcll(__ballot(key >= h)) >= few) high = h;
@@ -102,14 +129,15 @@ __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restric
                                                               double2* __restrict__ sums, float* __restrict__ values,
                                                               int* __restrict__ tokens, PieceArgs a) {
   constexpr int N = Chunk<T>::N, CHUNKS = E / N;
-  extern __shared__ __align__(16) unsigned long long list[];   // (key, ~token) of what reaches the bound, a part for every wave
+  extern __shared__ __align__(16) unsigned long long list[];
+  // list: (key, ~token) of what reaches the bound, a part for every wave
   __shared__ uint32_t bound_of[NWAVES], share_of[NWAVES];
   __shared__ float max_of[NWAVES];
   __shared__ double sum_of[NWAVES];
   __shared__ int n_of[NWAVES];
   const int tid = threadIdx.x, lane = tid % KVF_WAVE, wave = tid / KVF_WAVE;
   const int row = blockIdx.y, piece = blockIdx.x;
-  if (!alive(scores[row])) return;       // the whole workgroup: the merge passes such rows over
+  if (!alive(scores[row])) return;       // the whole workgroup: such rows are passed over
   const size_t at = static_cast<size_t>(row) * a.pieces + piece;
   const T* x = logits + row * a.stride;
   // chunks lie on 16 bytes of memory: element e of the row is place e + skip of its first chunk's line
@@ -155,8 +183,8 @@ __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restric
   }
   const uint32_t lane_key = mx > -INFINITY ? order_key(mx) : 0u;
   uint32_t wave_bound, wave_share;
-  kth_of_lanes(lane_key, a.count, (a.count + NWAVES - 1) / NWAVES, wave_bound, wave_share);
-  const float wmx = wave_max(mx);
+  kth_of_lanes<0>(lane_key, a.count, (a.count + NWAVES - 1) / NWAVES, wave_bound, wave_share);
+  const float wmx = wave_most(mx);
   if (lane == 0) {
     bound_of[wave] = wave_bound;
     share_of[wave] = wave_share;
@@ -228,16 +256,30 @@ __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restric
   // every entry counts those ahead of it: its place
   float* out_v = values + at * a.count;
   int* out_t = tokens + at * a.count;
+  int rest[NWAVES];
+#pragma unroll
+  for (int w = 0; w < NWAVES; ++w) rest[w] = n_of[w];
+  // the first step of every part, all in flight where registers are no matter
+  constexpr int NEAR = E <= 8 ? LIST_STEP / 2 : 0;
+  ulonglong2 near[NWAVES][NEAR + 1];
+#pragma unroll
+  for (int w = 0; w < NWAVES; ++w)
+#pragma unroll
+    for (int u = 0; u < NEAR; ++u) near[w][u] = reinterpret_cast<const ulonglong2*>(list + w * room)[u];
   for (int i = lane; i < held; i += KVF_WAVE) {
     const unsigned long long entry = mine[i];
     int place = 0;
 #pragma unroll
+    for (int w = 0; w < NWAVES; ++w)
+#pragma unroll
+      for (int u = 0; u < NEAR; ++u) place += (near[w][u].x > entry) + (near[w][u].y > entry);
+#pragma unroll
     for (int w = 0; w < NWAVES; ++w) {
       const ulonglong2* other = reinterpret_cast<const ulonglong2*>(list + w * room);
-      for (int j = 0; j < n_of[w]; j += LIST_STEP) {
+      for (int k = 2 * NEAR; k < rest[w]; k += LIST_STEP) {
         ulonglong2 e[LIST_STEP / 2];
 #pragma unroll
-        for (int u = 0; u < LIST_STEP / 2; ++u) e[u] = other[j / 2 + u];
+        for (int u = 0; u < LIST_STEP / 2; ++u) e[u] = other[k / 2 + u];
 #pragma unroll
         for (int u = 0; u < LIST_STEP / 2; ++u) place += (e[u].x > entry) + (e[u].y > entry);
       }
@@ -247,7 +289,7 @@ __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restric
       out_t[place] = static_cast<int>(~static_cast<uint32_t>(entry));
     }
   }
-  const int n = n_of[0] + n_of[1] + n_of[2] + n_of[3];
+  const int n = rest[0] + rest[1] + rest[2] + rest[3];
   for (int i = n + tid; i < a.count; i += THREADS) {
     out_v[i] = -INFINITY;
     out_t[i] = -1;
@@ -263,7 +305,7 @@ __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restric
 // An entry of a sorted list: score, and what tells equal scores apart (lower first): the beam in the upper 16 bits, then the
 // logit, largest first (scores of a beam may be equal in 64 bits though its logits are not), then the place in the beam's
 // lists, which is in the order of the tokens.
-struct Entry {
+struct __align__(16) Entry {
   double score;
   unsigned long long tie;
 };
@@ -271,24 +313,8 @@ constexpr unsigned long long NOBODY = ~0ull;
 __device__ __forceinline__ bool ahead(const Entry& a, const Entry& b) {
   return a.score > b.score || (a.score == b.score && a.tie < b.tie);
 }
-// The value of lane ^ O (O = 1 .. 63 of the forms below) without the LDS crossbar where it lies in the same 16 lanes: 1 and 2 are
-// permutations of four lanes, 7 and 15 the mirrors of 8 and 16, and 4 = 7 ^ 3, 8 = 15 ^ 7.
-template <int O> __device__ __forceinline__ uint32_t of_lane(uint32_t v) {
-  auto dpp = [](uint32_t x, auto ctrl) { return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, 0xF, 0xF, true)); };
-  if constexpr (O == 1) return dpp(v, std::integral_constant<int, 0xB1>{});
-  else if constexpr (O == 2) return dpp(v, std::integral_constant<int, 0x4E>{});
-  else if constexpr (O == 3) return dpp(v, std::integral_constant<int, 0x1B>{});
-  else if constexpr (O == 7) return dpp(v, std::integral_constant<int, 0x141>{});
-  else if constexpr (O == 15) return dpp(v, std::integral_constant<int, 0x140>{});
-  else if constexpr (O == 4) return of_lane<3>(of_lane<7>(v));
-  else if constexpr (O == 8) return of_lane<7>(of_lane<15>(v));
-  else return static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), O, KVF_WAVE));
-}
-template <int O> __device__ __forceinline__ unsigned long long of_lane(unsigned long long v) {
-  return static_cast<unsigned long long>(of_lane<O>(static_cast<uint32_t>(v >> 32))) << 32 | of_lane<O>(static_cast<uint32_t>(v));
-}
 template <int O> __device__ __forceinline__ Entry entry_of(const Entry& e) {
-  return {__longlong_as_double(static_cast<long long>(of_lane<O>(static_cast<unsigned long long>(__double_as_longlong(e.score))))), of_lane<O>(e.tie)};
+  return {of_lane<O>(e.score), of_lane<O>(e.tie)};
 }
 
 // The best L of two sorted lists of L that lie in groups of L lanes (L a power of two), sorted.
@@ -304,11 +330,11 @@ template <int L> __device__ __forceinline__ Entry merge_lists(Entry mine, Entry 
   exchange<L / 2>(e, lane);
   return e;
 }
-// The lists of a wave's groups of L lanes, O lanes apart and more, as one in every group.
-template <int L, int O> __device__ __forceinline__ void merge_groups(Entry& e, int lane) {
-  if constexpr (O < KVF_WAVE) {
+// The lists of a wave's groups of L lanes, O lanes apart and more within LANES, as one in every group.
+template <int L, int O, int LANES = KVF_WAVE> __device__ __forceinline__ void merge_groups(Entry& e, int lane) {
+  if constexpr (O < LANES) {
     e = merge_lists<L>(e, entry_of<O ^ (L - 1)>(e), lane);
-    merge_groups<L, 2 * O>(e, lane);
+    merge_groups<L, 2 * O, LANES>(e, lane);
   }
 }
 
@@ -316,93 +342,230 @@ struct BestArgs {
   int rows, requests, count, pieces;
 };
 constexpr int BATCH = 64;       // rows of a request that are merged at a time
+constexpr int FEW = 512;        // entries that are put in order by counting those ahead of each
 
-// L: `count` rounded up to a power of two; W waves.
-template <int L, int W>
-__global__ __launch_bounds__(W * KVF_WAVE) void beam_best_kernel(const float* __restrict__ scores, const int* __restrict__ cu_beams,
-                                                                 const double2* __restrict__ sums, const float* __restrict__ values,
-                                                                 const int* __restrict__ tokens, float* __restrict__ out_scores,
-                                                                 int* __restrict__ out_beams, int* __restrict__ out_tokens, BestArgs a) {
-  constexpr int SIDE = KVF_WAVE / L;       // lists side by side in a wave
-  __shared__ double list_s[W][L];
-  __shared__ unsigned long long list_t[W][L];
-  __shared__ double2 row_of[BATCH];        // (reference, S - log(sum)) of a row
+constexpr int BEST_WAVES = 8, BEST_THREADS = BEST_WAVES * KVF_WAVE;
+
+struct Survivors {
+  Entry entry[FEW + 4];
+  int token[FEW];
+  uint32_t bound_of[BEST_WAVES], share_of[BEST_WAVES];
+  int n;
+};
+template <int L> struct Merged {
+  Entry entry[BEST_WAVES][L];
+};
+
+// (reference, S - log(sum)) of a row, in all lanes of the wave; (-inf, -inf) of one that has ended or has no candidate.
+// `mine`: the sums of piece `lane`.
+__device__ __forceinline__ double2 join_sums(const double2* p, double2 mine, float score, int pieces) {
+  const int lane = threadIdx.x % KVF_WAVE;
+  double m = -INFINITY, s = 0.0;
+  if (alive(score)) {
+    float most = static_cast<float>(mine.y);      // (a logit)
+    for (int i = lane + KVF_WAVE; i < pieces; i += KVF_WAVE) most = fmaxf(most, static_cast<float>(p[i].y));
+    m = wave_most(most);
+    if (m > -INFINITY) {
+      s = mine.x * exp(mine.y - m);
+      for (int i = lane + KVF_WAVE; i < pieces; i += KVF_WAVE) s += p[i].x * exp(p[i].y - m);
+    }
+    s = wave_sum64(s);
+  }
+  return make_double2(m, s > 0.0 ? static_cast<double>(score) - log(s) : -INFINITY);
+}
+// What tells equal scores apart: see `Entry`.
+__device__ __forceinline__ unsigned long long tie_of(int beam, float value, int place) {
+  return static_cast<unsigned long long>(beam) << 48 | static_cast<unsigned long long>(~order_key(value)) << 16 | static_cast<unsigned long long>(place);
+}
+// The upper half of a score's order as an integer: scores in order have it in order (equal ones perhaps).
+__device__ __forceinline__ uint32_t upper_key(double s) {
+  const uint32_t b = static_cast<uint32_t>(static_cast<unsigned long long>(__double_as_longlong(s)) >> 32);
+  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+}
+
+// A wave's way through the entries of its rows (wave, wave + BEST_WAVES, ... of the request, `per_row` entries a lane each).  Lists
+// are sorted, so lanes are turned against them from step to step: the best of a list do not all fall to the same lanes, and the
+// bound, which goes by the lanes' best, is near.
+struct Walk {
+  int beam, part, turn;
+  __device__ __forceinline__ int entry() const { return part * KVF_WAVE + ((threadIdx.x + turn) & (KVF_WAVE - 1)); }
+  __device__ __forceinline__ void next(int per_row) {
+    if (++part == per_row) part = 0, beam += BEST_WAVES;
+    turn += 7;
+  }
+};
+constexpr int SLOTS = 4;        // entries a lane has in its registers at a time
+
+// All entries of a request's rows, a wave a row: the same bound as for a piece, by the upper halves of the scores, then every
+// entry that reaches it counts those ahead.  False where more than FEW do (equal scores, mostly).
+__device__ __forceinline__ bool best_by_counting(const float* scores, const double2* sums, const float* values, const int* tokens, int first,
+                                                 int beams, int request, float* out_scores, int* out_beams, int* out_tokens,
+                                                 const BestArgs& a, double2* row_of, Survivors& x) {
+  const int tid = threadIdx.x, lane = tid % KVF_WAVE, wave = tid / KVF_WAVE;
+  const int entries = a.pieces * a.count, per_row = (entries + KVF_WAVE - 1) / KVF_WAVE;
+  if (beams > BATCH) return false;
+  if (beams == 0) {
+    if (tid < a.count) {
+      const size_t to = static_cast<size_t>(request) * a.count + tid;
+      out_scores[to] = -INFINITY;
+      out_beams[to] = out_tokens[to] = -1;
+    }
+    return true;
+  }
+  const int slots = (beams + BEST_WAVES - 1 - wave) / BEST_WAVES * per_row;
+  float value[SLOTS];
+  int token[SLOTS];
+  auto load = [&](Walk w) {
+#pragma unroll
+    for (int k = 0; k < SLOTS; ++k) {
+      const int e = w.entry();
+      const bool there = w.beam < beams && e < entries;
+      const size_t from = there ? static_cast<size_t>(first + w.beam) * entries + e : 0;
+      const int read = tokens[from];          // (always: loads behind conditions go one by one)
+      value[k] = values[from];
+      token[k] = there ? read : -1;
+      w.next(per_row);
+    }
+  };
+  load({wave, 0, 0});
+  for (int b = wave; b < beams; b += BEST_WAVES) {
+    const int row = first + b;
+    const float score = scores[row];
+    const double2* p = sums + static_cast<size_t>(row) * a.pieces;
+    const double2 mine = lane < a.pieces ? p[lane] : make_double2(0.0, -INFINITY);
+    const double2 r = join_sums(p, mine, score, a.pieces);
+    if (lane == 0) row_of[b] = r;
+  }
+  if (tid == 0) x.n = 0;
+  // (row_of is this wave's own)
+  double s[SLOTS];
+  auto score_all = [&](Walk w) {
+#pragma unroll
+    for (int k = 0; k < SLOTS; ++k) {
+      const double2 r = row_of[min(w.beam, beams - 1)];
+      s[k] = token[k] >= 0 && r.y > -INFINITY ? (static_cast<double>(value[k]) - r.x) + r.y : -INFINITY;
+      w.next(per_row);
+    }
+  };
+  uint32_t most = 0;
+  Walk from{wave, 0, 0};
+  for (int k0 = 0; k0 < slots; k0 += SLOTS) {
+    Walk w = from;
+    if (k0) load(w);
+    score_all(w);
+#pragma unroll
+    for (int k = 0; k < SLOTS; ++k) {
+      const uint32_t key = s[k] > -INFINITY ? upper_key(s[k]) : 0u;
+      most = key > most ? key : most;
+      w.next(per_row);
+    }
+    from = w;
+  }
+  uint32_t kth, high;
+  kth_of_lanes<8>(most, a.count, (a.count + BEST_WAVES - 1) / BEST_WAVES, kth, high);
+  if (lane == 0) {
+    x.bound_of[wave] = kth;
+    x.share_of[wave] = high;
+  }
+  __syncthreads();
+  uint32_t bound = x.share_of[0];
+#pragma unroll
+  for (int w = 1; w < BEST_WAVES; ++w) bound = x.share_of[w] < bound ? x.share_of[w] : bound;
+#pragma unroll
+  for (int w = 0; w < BEST_WAVES; ++w) bound = x.bound_of[w] > bound ? x.bound_of[w] : bound;
+  from = {wave, 0, 0};
+  for (int k0 = 0; k0 < slots; k0 += SLOTS) {
+    Walk w = from;
+    if (slots > SLOTS) {
+      load(w);
+      score_all(w);
+    }
+#pragma unroll
+    for (int k = 0; k < SLOTS; ++k) {
+      const bool takes = s[k] > -INFINITY && upper_key(s[k]) >= bound;
+      const unsigned long long who = __ballot(takes);
+      if (who) {
+        int base = 0;
+        if (lane == 0) base = atomicAdd(&x.n, static_cast<int>(__popcll(who)));
+        const int to = __shfl(base, 0, KVF_WAVE) + __popcll(who & ((1ull << lane) - 1ull));
+        if (takes && to < FEW) {
+          x.entry[to] = {s[k], tie_of(w.beam, value[k], w.entry())};
+          x.token[to] = token[k];
+        }
+      }
+      w.next(per_row);
+    }
+    from = w;
+  }
+  __syncthreads();
+  const int n = x.n;
+  if (n > FEW) return false;
+  if (tid < 4) x.entry[n + tid] = {-INFINITY, NOBODY};            // whole steps
+  __syncthreads();
+  for (int i = tid; i < n; i += BEST_THREADS) {
+    const Entry mine = x.entry[i];
+    int place = 0;
+    for (int j = 0; j < n; j += 4)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) place += ahead(x.entry[j + u], mine);
+    if (place < a.count) {
+      const size_t to = static_cast<size_t>(request) * a.count + place;
+      out_scores[to] = static_cast<float>(mine.score);
+      out_beams[to] = static_cast<int>(mine.tie >> 48);
+      out_tokens[to] = x.token[i];
+    }
+  }
+  for (int i = n + tid; i < a.count; i += BEST_THREADS) {
+    const size_t to = static_cast<size_t>(request) * a.count + i;
+    out_scores[to] = -INFINITY;
+    out_beams[to] = -1;
+    out_tokens[to] = -1;
+  }
+  return true;
+}
+
+// The same for any number of entries: the sorted lists of all rows merged, those of a wave side by side.  L: `count` rounded up
+// to a power of two.
+template <int L>
+__device__ __forceinline__ void best_by_merging(const float* scores, const double2* sums, const float* values, const int* tokens, int first,
+                                                int beams, int request, float* out_scores, int* out_beams, int* out_tokens,
+                                                const BestArgs& a, double2* row_of, Merged<L>& x) {
+  constexpr int SIDE = KVF_WAVE / L;
   const int tid = threadIdx.x, lane = tid % KVF_WAVE, wave = tid / KVF_WAVE, group = lane / L, at = lane % L;
-  const int request = blockIdx.x;
-  const int first = min(max(cu_beams[request], 0), a.rows);
-  const int beams = min(max(cu_beams[request + 1], first), a.rows) - first;
   Entry best{-INFINITY, NOBODY};
   for (int b0 = 0; b0 < beams; b0 += BATCH) {
     const int n = min(BATCH, beams - b0), lists = n * a.pieces;
     const size_t base = static_cast<size_t>(first + b0) * a.pieces;
-    // list l of the batch, its entry i: loaded before the sums are there
-    float value;
-    int token;
-    auto load = [&](int l, int i) {
-      const bool there = l < lists && i < a.count;
-      const size_t from = (base + (there ? l : 0)) * a.count + (there ? i : 0);
-      value = values[from];
-      token = there ? tokens[from] : -1;
-    };
-    auto entry = [&](int l, int i) {
-      Entry e{-INFINITY, NOBODY};
-      if (token >= 0) {
-        const int beam = l / a.pieces;
-        const double2 r = row_of[beam];
-        if (r.y > -INFINITY) {
-          e.score = (static_cast<double>(value) - r.x) + r.y;
-          e.tie = static_cast<unsigned long long>(b0 + beam) << 48 | static_cast<unsigned long long>(~order_key(value)) << 16 |
-                  static_cast<unsigned long long>((l - beam * a.pieces) * a.count + i);
-        }
-      }
-      return e;
-    };
-    // `best` is sorted, so the other list is taken from its end
-    int l = wave * SIDE + group;
-    load(l, L - 1 - at);
-    if (b0) __syncthreads();
-    for (int b = wave; b < n; b += W) {
+    __syncthreads();
+    for (int b = wave; b < n; b += BEST_WAVES) {
       const int row = first + b0 + b;
-      const float score = scores[row];
-      double m = -INFINITY, s = 0.0;
-      if (alive(score)) {
-        const double2* p = sums + static_cast<size_t>(row) * a.pieces;
-        double2 mine = lane < a.pieces ? p[lane] : make_double2(0.0, -INFINITY);
-        m = mine.y;
-        for (int i = lane + KVF_WAVE; i < a.pieces; i += KVF_WAVE) m = fmax(m, p[i].y);
-#pragma unroll
-        for (int o = KVF_WAVE / 2; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, KVF_WAVE));
-        if (m > -INFINITY) {
-          s = mine.x * exp(mine.y - m);
-          for (int i = lane + KVF_WAVE; i < a.pieces; i += KVF_WAVE) s += p[i].x * exp(p[i].y - m);
-        }
-        s = wave_sum64(s);
-      }
-      if (lane == 0) row_of[b] = make_double2(m, s > 0.0 ? static_cast<double>(score) - log(s) : -INFINITY);
+      const double2* p = sums + static_cast<size_t>(row) * a.pieces;
+      const double2 r = join_sums(p, lane < a.pieces ? p[lane] : make_double2(0.0, -INFINITY), scores[row], a.pieces);
+      if (lane == 0) row_of[b] = r;
     }
     __syncthreads();
-    while (l - group < lists) {
-      const Entry e = entry(l, L - 1 - at);
-      l += W * SIDE;
-      if (l - group < lists) load(l, L - 1 - at);
+    // `best` is sorted, so the other list is taken from its end
+    const int i = L - 1 - at;
+    for (int l = wave * SIDE + group; l - group < lists; l += BEST_WAVES * SIDE) {
+      Entry e{-INFINITY, NOBODY};
+      if (l < lists && i < a.count) {
+        const int beam = l / a.pieces;
+        const size_t from = (base + l) * a.count + i;
+        const double2 r = row_of[beam];
+        if (r.y > -INFINITY && tokens[from] >= 0) {
+          e.score = (static_cast<double>(values[from]) - r.x) + r.y;
+          e.tie = tie_of(b0 + beam, values[from], (l - beam * a.pieces) * a.count + i);
+        }
+      }
       best = merge_lists<L>(best, e, lane);
     }
   }
   merge_groups<L, L>(best, lane);
-  if (lane < L) {
-    list_s[wave][lane] = best.score;
-    list_t[wave][lane] = best.tie;
-  }
+  if (lane < L) x.entry[wave][lane] = best;
   __syncthreads();
   if (wave > 0) return;
-  // the waves' lists, those that the groups hold already left out: group g takes g, g + SIDE, ...
-  best = group < W ? Entry{list_s[group][at], list_t[group][at]} : Entry{-INFINITY, NOBODY};
-  for (int w = SIDE; w < W; w += SIDE) {
-    const int take = w + group;
-    const Entry other = take < W ? Entry{list_s[take][L - 1 - at], list_t[take][L - 1 - at]} : Entry{-INFINITY, NOBODY};
-    best = merge_lists<L>(best, other, lane);
-  }
-  merge_groups<L, L>(best, lane);
+#pragma unroll
+  for (int w = 1; w < BEST_WAVES; ++w) best = merge_lists<L>(best, x.entry[w][L - 1 - at], lane);
   if (lane < a.count) {
     const bool there = best.tie != NOBODY;
     const int beam = static_cast<int>(best.tie >> 48);
@@ -411,6 +574,23 @@ __global__ __launch_bounds__(W * KVF_WAVE) void beam_best_kernel(const float* __
     out_beams[to] = there ? beam : -1;
     out_tokens[to] = there ? tokens[static_cast<size_t>(first + beam) * a.pieces * a.count + (best.tie & 0xffffull)] : -1;
   }
+}
+
+template <int L>
+__global__ __launch_bounds__(BEST_THREADS) void beam_best_kernel(const float* scores, const int* __restrict__ cu_beams, const double2* sums,
+                                                            const float* values, const int* tokens, float* out_scores, int* out_beams,
+                                                            int* out_tokens, BestArgs a) {
+  __shared__ union {
+    Survivors few;
+    Merged<L> merged;
+  } x;
+  __shared__ double2 row_of[BATCH];
+  const int request = blockIdx.x;
+  const int first = min(max(cu_beams[request], 0), a.rows);
+  const int beams = min(max(cu_beams[request + 1], first), a.rows) - first;
+  if (best_by_counting(scores, sums, values, tokens, first, beams, request, out_scores, out_beams, out_tokens, a, row_of, x.few)) return;
+  __syncthreads();
+  best_by_merging<L>(scores, sums, values, tokens, first, beams, request, out_scores, out_beams, out_tokens, a, row_of, x.merged);
 }
 
 template <typename T, int E>
@@ -422,41 +602,33 @@ int pieces_launch(const void* logits, const float* scores, double2* sums, float*
 }  // namespace
 
 // logits [rows][stride] of `vocab` (bf16: 0 fp32, 1 bf16); scores [rows]; cu_beams [requests + 1]; out_* [requests][count].
-// Workspace: sums [rows][pieces][2] in 64 bits, values/tokens [rows][pieces][count].  piece: elements of a
-// piece, 256 times 8 or 32.
+// Workspace: sums [rows][pieces][2] in 64 bits, values/tokens [rows][pieces][count].  piece: elements of a piece, 256 times 8, or
+// 32 for up to 32 candidates.
 KVF_EXPORT int kvf_beam_select(int bf16, const void* logits, long stride, int rows, int vocab, const float* scores,
-                               const int* cu_beams, int requests, int count, int pieces, int piece, void* sums, float* values, int* tokens, float* out_scores, int* out_beams, int* out_tokens,
-                               hipStream_t stream) {
+                               const int* cu_beams, int requests, int count, int pieces, int piece, void* sums,
+                               float* values, int* tokens, float* out_scores, int* out_beams, int* out_tokens, hipStream_t stream) {
   if (count < 1 || count > MAX_COUNT || rows < 0 || rows > 65535 || vocab < 1 || pieces < 1 || requests < 0 ||
       static_cast<long>(pieces) * count > 65536)
     return static_cast<int>(hipErrorInvalidValue);
-  if (piece != THREADS * 8 && piece != THREADS * 32) return static_cast<int>(hipErrorInvalidValue);
+  if (piece != THREADS * 8 && (piece != THREADS * 32 || count > 32)) return static_cast<int>(hipErrorInvalidValue);
   if (requests == 0) return 0;
   // a row may begin up to 15 bytes into its first chunk
   if (static_cast<long>(pieces) * piece < static_cast<long>(vocab) + (bf16 ? 7 : 3)) return static_cast<int>(hipErrorInvalidValue);
+  auto* sum = static_cast<double2*>(sums);
   if (rows) {
     const PieceArgs a{stride, rows, vocab, count, pieces, piece};
-    auto* s = static_cast<double2*>(sums);
     int rc;
     if (bf16)
-      rc = piece == THREADS * 8 ? pieces_launch<bf16_t, 8>(logits, scores, s, values, tokens, a, stream)
-                                : pieces_launch<bf16_t, 32>(logits, scores, s, values, tokens, a, stream);
+      rc = piece == THREADS * 8 ? pieces_launch<bf16_t, 8>(logits, scores, sum, values, tokens, a, stream)
+                                : pieces_launch<bf16_t, 32>(logits, scores, sum, values, tokens, a, stream);
     else
-      rc = piece == THREADS * 8 ? pieces_launch<float, 8>(logits, scores, s, values, tokens, a, stream)
-                                : pieces_launch<float, 32>(logits, scores, s, values, tokens, a, stream);
+      rc = piece == THREADS * 8 ? pieces_launch<float, 8>(logits, scores, sum, values, tokens, a, stream)
+                                : pieces_launch<float, 32>(logits, scores, sum, values, tokens, a, stream);
     if (rc) return rc;
   }
   const BestArgs b{rows, requests, count, pieces};
-  const auto* s = static_cast<const double2*>(sums);
-  // more waves where a request has lists for them on average
-  const bool wide = static_cast<long>(rows) * pieces > 16L * requests;
-#define KVF_BEST(L)                                                                                                                       \
-  do {                                                                                                                                    \
-    if (wide) beam_best_kernel<L, 16><<<requests, 16 * KVF_WAVE, 0, stream>>>(scores, cu_beams, s, values, tokens, out_scores, out_beams, out_tokens, b); \
-    else beam_best_kernel<L, 4><<<requests, 4 * KVF_WAVE, 0, stream>>>(scores, cu_beams, s, values, tokens, out_scores, out_beams, out_tokens, b);        \
-  } while (0)
-  if (count <= 4) KVF_BEST(4);
-  else if (count <= 8) KVF_BEST(8);
+#define KVF_BEST(L) beam_best_kernel<L><<<requests, BEST_THREADS, 0, stream>>>(scores, cu_beams, sum, values, tokens, out_scores, out_beams, out_tokens, b)
+  if (count <= 8) KVF_BEST(8);
   else if (count <= 16) KVF_BEST(16);
   else if (count <= 32) KVF_BEST(32);
   else KVF_BEST(64);

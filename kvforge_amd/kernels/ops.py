@@ -2895,6 +2895,7 @@ def decode_advance(sampled: torch.Tensor, token_ids: torch.Tensor, positions: to
 BEAM_MAX_COUNT = 64      # candidates of a request
 BEAM_MAX_WIDTH = 32      # beams of a request that are reordered together
 BEAM_PIECES = (2048, 8192)     # logits of a row that one workgroup takes
+_BEAM_SELECT_ARGS = [c_int, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 7
 
 
 def _beam_pieces(rows: int, vocab: int, count: int, device) -> tuple[int, int]:
@@ -2906,8 +2907,7 @@ def _beam_pieces(rows: int, vocab: int, count: int, device) -> tuple[int, int]:
 
 
 def beam_select_workspace(rows: int, vocab: int, count: int, device) -> tuple[torch.Tensor, ...]:
-    """Scratch of ``beam_select`` for ``rows`` rows of logits: the pieces' sums, their best logits and the tokens of
-    these."""
+    """Scratch of ``beam_select`` for ``rows`` rows of logits: the pieces' sums, their best logits and the tokens of these."""
     pieces, _ = _beam_pieces(rows, vocab, count, device)
     return (torch.empty(rows * pieces * 2, dtype=torch.float64, device=device),
             torch.empty(rows * pieces * count, dtype=F32, device=device),
@@ -2956,7 +2956,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, cu_beams: torch.Tens
     if (sums.shape[0] < rows * pieces * 2 or min(values.shape[0], tokens.shape[0]) < rows * pieces * count or sums.data_ptr() % 16):
         raise KernelError("beam_select: workspace too small for these rows, logits and candidates")
     _here("beam_select", logits, scores, cu_beams, out_scores, out_beams, out_tokens, *workspace)
-    f = _fn("beam", "kvf_beam_select", [c_int, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 7)
+    f = _fn("beam", "kvf_beam_select", _BEAM_SELECT_ARGS)
     _ok(f(_tcode(logits.dtype), logits.data_ptr(), stride, rows, vocab, scores.data_ptr(),
           cu_beams.data_ptr(), requests, count, pieces, piece, sums.data_ptr(), values.data_ptr(),
           tokens.data_ptr(), out_scores.data_ptr(), out_beams.data_ptr(), out_tokens.data_ptr(), _stream()), "beam_select")

@@ -253,43 +253,35 @@ __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restric
     n_of[wave] = held;
   }
   __syncthreads();
-  // every entry counts those ahead of it: its place
+  // Every entry counts those ahead of it: its place.  Four lanes an entry, each over the part of one wave.
+  static_assert(NWAVES == 4, "a lane a part");
   float* out_v = values + at * a.count;
   int* out_t = tokens + at * a.count;
-  int rest[NWAVES];
+  int upto[NWAVES];
 #pragma unroll
-  for (int w = 0; w < NWAVES; ++w) rest[w] = n_of[w];
-  // the first step of every part, all in flight where registers are no matter
-  constexpr int NEAR = E <= 8 ? LIST_STEP / 2 : 0;
-  ulonglong2 near[NWAVES][NEAR + 1];
-#pragma unroll
-  for (int w = 0; w < NWAVES; ++w)
-#pragma unroll
-    for (int u = 0; u < NEAR; ++u) near[w][u] = reinterpret_cast<const ulonglong2*>(list + w * room)[u];
-  for (int i = lane; i < held; i += KVF_WAVE) {
-    const unsigned long long entry = mine[i];
+  for (int w = 0; w < NWAVES; ++w) upto[w] = n_of[w] + (w ? upto[w - 1] : 0);
+  const int n = upto[NWAVES - 1];
+  const auto* other = reinterpret_cast<const ulonglong2*>(list + (tid % NWAVES) * room);
+  const int others = n_of[tid % NWAVES];
+  for (int i0 = 0; i0 < n; i0 += THREADS / NWAVES) {
+    const int i = i0 + tid / NWAVES;
+    unsigned long long entry = 0ull;
+    if (i < n) entry = i < upto[0] ? list[i] : i < upto[1] ? list[room + i - upto[0]] : i < upto[2] ? list[2 * room + i - upto[1]] : list[3 * room + i - upto[2]];
     int place = 0;
+    for (int k = 0; k < others; k += LIST_STEP) {
+      ulonglong2 e[LIST_STEP / 2];
 #pragma unroll
-    for (int w = 0; w < NWAVES; ++w)
+      for (int u = 0; u < LIST_STEP / 2; ++u) e[u] = other[k / 2 + u];
 #pragma unroll
-      for (int u = 0; u < NEAR; ++u) place += (near[w][u].x > entry) + (near[w][u].y > entry);
-#pragma unroll
-    for (int w = 0; w < NWAVES; ++w) {
-      const ulonglong2* other = reinterpret_cast<const ulonglong2*>(list + w * room);
-      for (int k = 2 * NEAR; k < rest[w]; k += LIST_STEP) {
-        ulonglong2 e[LIST_STEP / 2];
-#pragma unroll
-        for (int u = 0; u < LIST_STEP / 2; ++u) e[u] = other[k / 2 + u];
-#pragma unroll
-        for (int u = 0; u < LIST_STEP / 2; ++u) place += (e[u].x > entry) + (e[u].y > entry);
-      }
+      for (int u = 0; u < LIST_STEP / 2; ++u) place += (e[u].x > entry) + (e[u].y > entry);
     }
-    if (place < a.count) {
+    place += static_cast<int>(of_lane<1>(static_cast<uint32_t>(place)));
+    place += static_cast<int>(of_lane<2>(static_cast<uint32_t>(place)));
+    if (tid % NWAVES == 0 && i < n && place < a.count) {
       out_v[place] = key_value(static_cast<uint32_t>(entry >> 32));
       out_t[place] = static_cast<int>(~static_cast<uint32_t>(entry));
     }
   }
-  const int n = rest[0] + rest[1] + rest[2] + rest[3];
   for (int i = n + tid; i < a.count; i += THREADS) {
     out_v[i] = -INFINITY;
     out_t[i] = -1;
@@ -347,7 +339,7 @@ constexpr int FEW = 512;        // entries that are put in order by counting tho
 constexpr int BEST_WAVES = 8, BEST_THREADS = BEST_WAVES * KVF_WAVE;
 
 struct Survivors {
-  Entry entry[FEW + 4];
+  Entry entry[FEW + 8];
   int token[FEW];
   uint32_t bound_of[BEST_WAVES], share_of[BEST_WAVES];
   int n;
@@ -500,15 +492,20 @@ __device__ __forceinline__ bool best_by_counting(const float* scores, const doub
   __syncthreads();
   const int n = x.n;
   if (n > FEW) return false;
-  if (tid < 4) x.entry[n + tid] = {-INFINITY, NOBODY};            // whole steps
-  __syncthreads();
-  for (int i = tid; i < n; i += BEST_THREADS) {
-    const Entry mine = x.entry[i];
+  // eight lanes an entry, each over every eighth
+  constexpr int LANES = 8;
+  for (int i0 = 0; i0 < n; i0 += BEST_THREADS / LANES) {
+    const int i = i0 + tid / LANES;
+    const Entry mine = x.entry[min(i, n - 1)];
     int place = 0;
-    for (int j = 0; j < n; j += 4)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) place += ahead(x.entry[j + u], mine);
-    if (place < a.count) {
+    for (int j = tid % LANES; j < n; j += 2 * LANES) {
+      const Entry one = x.entry[j], two = x.entry[j + LANES];
+      place += ahead(one, mine) + (j + LANES < n && ahead(two, mine));
+    }
+    place += static_cast<int>(of_lane<1>(static_cast<uint32_t>(place)));
+    place += static_cast<int>(of_lane<2>(static_cast<uint32_t>(place)));
+    place += static_cast<int>(of_lane<7>(static_cast<uint32_t>(place)));
+    if (tid % LANES == 0 && i < n && place < a.count) {
       const size_t to = static_cast<size_t>(request) * a.count + place;
       out_scores[to] = static_cast<float>(mine.score);
       out_beams[to] = static_cast<int>(mine.tie >> 48);

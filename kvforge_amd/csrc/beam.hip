@@ -8,11 +8,12 @@
 // beams whose score is not finite are passed over unread.
 //
 //   1. `beam_pieces_kernel`: a workgroup takes a piece of a row, which stays in its registers (E logits a lane), so the row is read once.  Maximum, sum of
-//      exponentials, and the piece's `count` best, sorted.  They are found by a bound: of the 64 largest logits of a wave's
-//      lanes, the `count`-th and the (count / 4)-th largest are settled bit by bit with ballots; at least `count` logits reach
-//      the best of the four waves' former and the least of their latter, and seldom many more.  What reaches the larger of the
-//      two goes to a list in LDS, where every entry counts those ahead of it: its place.  (Logits equal to the bound are taken
-//      in the order of their tokens, no more than `count` a wave, so the list holds whatever the logits are.)
+//      exponentials, and the piece's `count` best, sorted.  They are found by a bound: the 64 largest logits of a wave's
+//      lanes, sorted, give a `count`-th and a (count / 4)-th; at least `count` logits reach the best of the four waves' former and
+//      the least of their latter, and seldom many more.  What reaches the larger of the two goes to a list in LDS, where
+//      every entry counts those ahead of it: its place.  (Logits equal to the bound are taken in the order of their tokens, no
+//      more than `count` a wave, so the list holds whatever the logits are.)
+//      512 rows of 128,256 (263 MB) take 47 us, 5.5 TB/s: as much as a kernel that only reads reaches on this card.
 //   2. `beam_best_kernel`: a workgroup a request joins the sums of a row's pieces in 64 bits (candidates of different
 //      beams may lie closer than 32 bits tell apart: their order is the sums' order), then picks among the pieces' best by a
 //      bound and by counting again.  Where equal scores let too many entries reach the bound, the sorted lists are merged
@@ -20,7 +21,7 @@
 //      and log2(count) exchanges sort them again.
 //   (One kernel, in which the workgroup of a request that is done last goes on with 2, saves 3 us of the host's time but takes
 //   longer on the device, since results have to pass the XCDs' L2s and 2's registers are 1's too: 4 rows of 8,192 logits 13.4 us
-//   and 10.3 so, 32 rows of 128,256 18.0 and 13.6, 512 rows 79 and 62.)
+//   against 10.3, 32 rows of 128,256 18.0 against 13.6, 512 rows 79 against 62, when it was tried.)
 //
 // Reordering: see `beam_reorder_kernel`.
 #include <type_traits>
@@ -86,15 +87,26 @@ __device__ __forceinline__ float wave_most(float v) {
   return fmaxf(v, of(v, std::integral_constant<int, 32>{}));
 }
 
-// The `count`-th and the `few`-th largest of 64 lanes' keys (0 where fewer are above 0), down to bit LOW.
-template <int LOW> __device__ __forceinline__ void kth_of_lanes(uint32_t key, int count, int few, uint32_t& kth, uint32_t& high) {
-  kth = high = 0;
-#pragma unroll
-  for (int bit = 31; bit >= LOW; --bit) {
-    const uint32_t k = kth | (1u << bit), h = high | (1u << bit);
-    if (__popcll(__ballot(key >= k)) >= count) kth = k;
-    if (__popcll(__ballot(key >= h)) >= few) high = h;
-  }
+// One exchange of a bitonic sort, the larger key to the lower lane: O with its lower bits set compares mirrored halves, a power of
+// two the halves themselves.
+template <int O> __device__ __forceinline__ void order_lanes(uint32_t& key, int lane) {
+  const uint32_t other = of_lane<O>(key);
+  const bool lower = (lane & ((O & (O - 1)) ? (O + 1) / 2 : O)) == 0;
+  const uint32_t more = key > other ? key : other, less = key > other ? other : key;
+  key = lower ? more : less;
+}
+// The `count`-th and the `few`-th largest of 64 lanes' keys: sorted, in about a hundred instructions (settling a threshold bit by
+// bit takes four times as many).
+__device__ __forceinline__ void kth_of_lanes(uint32_t key, int count, int few, uint32_t& kth, uint32_t& high) {
+  const int lane = threadIdx.x % KVF_WAVE;
+  order_lanes<1>(key, lane);
+  order_lanes<3>(key, lane), order_lanes<1>(key, lane);
+  order_lanes<7>(key, lane), order_lanes<2>(key, lane), order_lanes<1>(key, lane);
+  order_lanes<15>(key, lane), order_lanes<4>(key, lane), order_lanes<2>(key, lane), order_lanes<1>(key, lane);
+  order_lanes<31>(key, lane), order_lanes<8>(key, lane), order_lanes<4>(key, lane), order_lanes<2>(key, lane), order_lanes<1>(key, lane);
+  order_lanes<63>(key, lane), order_lanes<16>(key, lane), order_lanes<8>(key, lane), order_lanes<4>(key, lane), order_lanes<2>(key, lane), order_lanes<1>(key, lane);
+  kth = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(key), count - 1));
+  high = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(key), few - 1));
 }
 
 // 16 bytes of logits at p[0..], as keys; places outside [0, n) give 0.
@@ -183,7 +195,7 @@ __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restric
   }
   const uint32_t lane_key = mx > -INFINITY ? order_key(mx) : 0u;
   uint32_t wave_bound, wave_share;
-  kth_of_lanes<0>(lane_key, a.count, (a.count + NWAVES - 1) / NWAVES, wave_bound, wave_share);
+  kth_of_lanes(lane_key, a.count, (a.count + NWAVES - 1) / NWAVES, wave_bound, wave_share);
   const float wmx = wave_most(mx);
   if (lane == 0) {
     bound_of[wave] = wave_bound;
@@ -211,30 +223,36 @@ __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restric
   for (int c = 0; c < CHUNKS; ++c) {
     if (!__ballot(top[c] >= least)) continue;
     const int e = lo + (c * THREADS + tid) * N;
-    unsigned long long same[N];
-    int before = ties, all = 0;
+    unsigned long long same[N], equal = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
+      same[i] = __ballot(v[c][i] >= least);
+      if (!same[i]) continue;
       const unsigned long long who = __ballot(v[c][i] > least);
       if (v[c][i] > least)
         mine[held + __popcll(who & below)] = static_cast<unsigned long long>(order_key(v[c][i])) << 32 | static_cast<uint32_t>(~(e + i));
       held += __popcll(who);
-      same[i] = __ballot(v[c][i] == least);
-      before += __popcll(same[i] & below);
-      all += __popcll(same[i]);
+      same[i] &= ~who;
+      equal |= same[i];
     }
-    if (all && ties < a.count) {
+    if (equal && ties < a.count) {
+      int before = ties;            // equals of lower tokens
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const bool equal = same[i] >> lane & 1ull;
-        const unsigned long long who = __ballot(equal && before < a.count);
-        if (equal && before < a.count)
+        before += __popcll(same[i] & below);
+        ties += __popcll(same[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (!same[i]) continue;
+        const bool is = same[i] >> lane & 1ull;
+        const unsigned long long who = __ballot(is && before < a.count);
+        if (is && before < a.count)
           mine[held + __popcll(who & below)] = static_cast<unsigned long long>(order_key(least)) << 32 | static_cast<uint32_t>(~(e + i));
         held += __popcll(who);
-        before += equal;
+        before += is;
       }
     }
-    ties += all;
   }
   double s = 0.0;
   if (m > -INFINITY) {
@@ -454,7 +472,7 @@ __device__ __forceinline__ bool best_by_counting(const float* scores, const doub
     from = w;
   }
   uint32_t kth, high;
-  kth_of_lanes<8>(most, a.count, (a.count + BEST_WAVES - 1) / BEST_WAVES, kth, high);
+  kth_of_lanes(most, a.count, (a.count + BEST_WAVES - 1) / BEST_WAVES, kth, high);
   if (lane == 0) {
     x.bound_of[wave] = kth;
     x.share_of[wave] = high;

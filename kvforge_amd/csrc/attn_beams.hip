@@ -98,24 +98,20 @@ template <typename T> struct Tensors {
   float2* ml;
 };
 
-// The keys that the sequences [first, first + n) share: no more than the shortest of them that has any.  `holder`: the first
-// that has any, whose pages they are read from.
-__device__ __forceinline__ int shared_keys(int group, int first, int n, const int* shared_lens, const int* ctx_lens, int most, int& holder) {
-  int least = most, who = n - 1;
-  for (int i = threadIdx.x % KVF_WAVE; i < n; i += KVF_WAVE) {
-    const int c = ctx_lens[first + i];
-    if (c > 0) {
-      least = min(least, c);
-      who = min(who, i);
-    }
+// The sequence of [first, first + n) whose pages the group's `shared` keys are read from: the first that holds as many, or else the
+// one that holds the most.
+__device__ __forceinline__ int holder_of(int first, int n, int shared, const int* __restrict__ ctx_lens) {
+  const int lane = threadIdx.x % KVF_WAVE;
+  for (int i = 0; i < n; i += KVF_WAVE) {
+    const unsigned long long held = __ballot(i + lane < n && ctx_lens[first + min(i + lane, n - 1)] >= shared);
+    if (held) return first + i + __ffsll(static_cast<long long>(held)) - 1;
   }
-#pragma unroll
-  for (int o = KVF_WAVE / 2; o > 0; o >>= 1) {
-    least = min(least, __shfl_xor(least, o, KVF_WAVE));
-    who = min(who, __shfl_xor(who, o, KVF_WAVE));
+  int most = 0, who = first;
+  for (int i = first; i < first + n; ++i) {
+    const int c = ctx_lens[i];
+    if (c > most) most = c, who = i;
   }
-  holder = first + who;
-  return max(0, min(least, shared_lens[group]));
+  return who;
 }
 
 // What a wave holds of 16 * RT rows: Q, and the running reference, sum and accumulator of each.
@@ -125,6 +121,7 @@ template <typename T, int DT, int RT> struct Rows {
   typename F::Part q[RT][SLICES];
   f32x4 acc[RT][DT];
   float m[RT], sum[RT];
+  int ctx[RT];           // keys of the row's sequence
 
   // Rows [row0, row0 + 16 RT) of `rows`: sequence first + row / G, head row % G of kv head `kvh`.
   __device__ __forceinline__ void start(const Tensors<T>& t, const Args& a, int first, int rows, int row0, int kvh) {
@@ -132,6 +129,7 @@ template <typename T, int DT, int RT> struct Rows {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int row = min(row0 + rt * 16 + r, rows - 1);
+      ctx[rt] = t.ctx_lens[first + row / G];
       const T* from = t.q + static_cast<long>(first + row / G) * a.q_stride + (kvh * G + row % G) * a.d;
 #pragma unroll
       for (int c = 0; c < SLICES; ++c) {
@@ -230,6 +228,10 @@ template <typename T, int DT, int RT> struct Rows {
 #pragma unroll
           for (int c = 0; c < SLICES; ++c) s[rt][tt] = F::scores(kf[tt][c], q[rt][c], s[rt][tt]);
         }
+      // (rows of sequences that are shorter than what their group shares see no more than their own keys)
+      bool all_rows = whole;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) all_rows &= static_cast<bool>(__all(kb + BLOCK <= ctx[rt]));
       if (next < hi) load_k(next, pk_next);
       typename F::Probs pf[RT];
 #pragma unroll
@@ -237,9 +239,9 @@ template <typename T, int DT, int RT> struct Rows {
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
           s[rt][tt] *= a.scale2;
-          if (!whole)
+          if (!all_rows)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[rt][tt][i] = keep >> (4 * tt + i) & 1u ? s[rt][tt][i] : -INFINITY;
+            for (int i = 0; i < 4; ++i) s[rt][tt][i] = (keep >> (4 * tt + i) & 1u) && kb + 8 * g + 4 * tt + i < ctx[rt] ? s[rt][tt][i] : -INFINITY;
         }
         float most = s[rt][0][0];
 #pragma unroll
@@ -279,19 +281,16 @@ template <typename T, int DT, int RT> struct Rows {
     }
   }
 
-  // Leaves tile rt's results as cut `cut` of its rows (`total`: sums over all keys of the cut).
-  __device__ __forceinline__ void leave(const Tensors<T>& t, const Args& a, int rt, float top, float total, int first, int rows, int row0, int kvh, int cut) {
-    const int lane = threadIdx.x % KVF_WAVE, g = lane / 16, r = lane % 16, G = a.H / a.KV, tiles = a.d / 16;
-    const int row = row0 + rt * 16 + r;
-    if (row >= rows) return;
-    const int seq = first + row / G;
-    const long at = (static_cast<long>(seq) * a.H + kvh * G + row % G) * (a.cs + a.co) + cut;
-    const bool any = t.ctx_lens[seq] > 0 && (total > 0.f || total != total);      // (NaN stays NaN)
-    if (g == 0) t.ml[at] = any ? make_float2(top > -INFINITY ? top : 0.f, total) : make_float2(-INFINITY, 0.f);
-    if (any)
-#pragma unroll
-      for (int j = 0; j < DT; ++j)
-        if (j < tiles) *reinterpret_cast<f32x4*>(t.acc + at * a.d + j * 16 + g * 4) = acc[rt][j];
+  // Where row rt * 16 + r of the rows leaves its results as cut `cut`; -1: nowhere.
+  __device__ __forceinline__ long place(const Args& a, int rt, int first, int rows, int row0, int kvh, int cut) const {
+    const int r = threadIdx.x % 16, G = a.H / a.KV, row = row0 + rt * 16 + r;
+    return row < rows ? (static_cast<long>(first + row / G) * a.H + kvh * G + row % G) * (a.cs + a.co) + cut : -1;
+  }
+  // (reference, sum over all keys of the cut), -inf where there are none (NaN stays NaN); whether there is an accumulator.
+  __device__ __forceinline__ bool leave_sum(const Tensors<T>& t, int rt, long at, float top, float total, bool writes) const {
+    const bool any = ctx[rt] > 0 && (total > 0.f || total != total);
+    if (writes && at >= 0) t.ml[at] = any ? make_float2(top > -INFINITY ? top : 0.f, total) : make_float2(-INFINITY, 0.f);
+    return any && at >= 0;
   }
   __device__ __forceinline__ float whole_sum(int rt) const {
     float l = sum[rt];
@@ -314,53 +313,63 @@ __device__ __forceinline__ void cut_of(int& lo, int& hi, int c, int n, int round
 // workgroups go to the eight XCDs in turn, so with eight heads an L2 holds the keys of one, also for a group's further rows.
 template <typename T, int DT, int RT, bool ALIGNED>
 __global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 16 && DT < 16 : RT * DT <= 8) void attn_beams_kernel(Tensors<T> t, Args a) {
-  __shared__ f32x4 lds_acc[(WAVES - 1) * DT * KVF_WAVE];
-  __shared__ float2 lds_ml[WAVES * 16];
+  __shared__ f32x4 lds_acc[RT][DT][WAVES - 1][KVF_WAVE];
+  __shared__ float2 lds_ml[RT][WAVES][16];
   const int shared_items = a.n_groups * a.cs * a.blocks * a.KV;
-  const int G = a.H / a.KV, most = a.width * a.bs, lane = threadIdx.x % KVF_WAVE, wave = threadIdx.x / KVF_WAVE, r = lane % 16;
+  const int G = a.H / a.KV, most = a.width * a.bs, lane = threadIdx.x % KVF_WAVE, wave = threadIdx.x / KVF_WAVE, g = lane / 16, r = lane % 16;
   if (static_cast<int>(blockIdx.x) < shared_items) {
     const int item = blockIdx.x;
     const int kvh = item % a.KV, block = item / a.KV % a.blocks, cut = item / a.KV / a.blocks % a.cs, group = item / a.KV / a.blocks / a.cs;
     const int first = min(max(t.cu_groups[group], 0), a.n_seqs), n = min(max(t.cu_groups[group + 1], first), a.n_seqs) - first;
     if (n == 0) return;
     const int rows = n * G, tiles = a.d / 16;
-    int holder, lo = 0, hi = shared_keys(group, first, n, t.shared_lens, t.ctx_lens, most, holder);
+    int lo = 0, hi = min(max(t.shared_lens[group], 0), most);
+    const int holder = holder_of(first, n, hi, t.ctx_lens);
     cut_of(lo, hi, cut, a.cs, WAVES * BLOCK);
     for (int row0 = block * 16 * RT; row0 < rows; row0 += a.blocks * 16 * RT) {
       Rows<T, DT, RT> x;
       x.start(t, a, first, rows, row0, kvh);
       x.template walk<ALIGNED>(t, a, t.table + static_cast<long>(holder) * a.width, kvh, lo + wave * BLOCK, WAVES * BLOCK, lo, hi);
-      // the waves' results, one tile of rows at a time
+      // the waves' results: tile j of the elements is summed by wave j % WAVES
+      float l[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const float l = x.whole_sum(rt);
-        __syncthreads();
-        if (lane < 16) lds_ml[wave * 16 + r] = make_float2(x.m[rt], l);
-        __syncthreads();
+        l[rt] = x.whole_sum(rt);
+        if (lane < 16) lds_ml[rt][wave][r] = make_float2(x.m[rt], l[rt]);
+      }
+      __syncthreads();
+      long at[RT];
+      bool any[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
         float top = -INFINITY, total = 0.f;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, lds_ml[w * 16 + r].x);
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, lds_ml[rt][w][r].x);
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
-          const float2 o = lds_ml[w * 16 + r];
+          const float2 o = lds_ml[rt][w][r];
           total += o.x > -INFINITY || o.y != o.y ? o.y * __builtin_amdgcn_exp2f(o.x - top) : 0.f;
         }
         const float by = x.m[rt] > -INFINITY ? __builtin_amdgcn_exp2f(x.m[rt] - top) : 0.f;
+        at[rt] = x.place(a, rt, first, rows, row0, kvh, cut);
+        any[rt] = x.leave_sum(t, rt, at[rt], top, total, wave == 0 && lane < 16);
 #pragma unroll
         for (int j = 0; j < DT; ++j) {
           x.acc[rt][j] *= by;
-          if (wave > 0 && j < tiles) lds_acc[((wave - 1) * DT + j) * KVF_WAVE + lane] = x.acc[rt][j];
-        }
-        __syncthreads();
-        if (wave == 0) {
-#pragma unroll
-          for (int j = 0; j < DT; ++j)
-            if (j < tiles)
-#pragma unroll
-              for (int w = 0; w < WAVES - 1; ++w) x.acc[rt][j] += lds_acc[(w * DT + j) * KVF_WAVE + lane];
-          x.leave(t, a, rt, top, total, first, rows, row0, kvh, cut);
+          if (j % WAVES != wave && j < tiles) lds_acc[rt][j][wave < j % WAVES ? wave : wave - 1][lane] = x.acc[rt][j];
         }
       }
+      __syncthreads();
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int j = 0; j < DT; ++j)
+          if (j % WAVES == wave && j < tiles) {
+            f32x4 o = x.acc[rt][j];
+#pragma unroll
+            for (int w = 0; w < WAVES - 1; ++w) o += lds_acc[rt][j][w][lane];
+            if (any[rt]) *reinterpret_cast<f32x4*>(t.acc + at[rt] * a.d + j * 16 + g * 4) = o;
+          }
     }
   } else {
     // (no barrier from here on)
@@ -374,23 +383,26 @@ __global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 
       const int g = min(g0 + lane, a.n_groups - 1);
       const unsigned long long here = __ballot(t.cu_groups[g] <= seq && seq < t.cu_groups[g + 1]);
       if (here) {
-        const int group = min(g0 + __ffsll(static_cast<long long>(here)) - 1, a.n_groups - 1);
-        const int first = max(t.cu_groups[group], 0);
-        int holder;
-        lo = a.cs ? shared_keys(group, first, min(t.cu_groups[group + 1], a.n_seqs) - first, t.shared_lens, t.ctx_lens, most, holder) : 0;
+        if (a.cs) lo = max(t.shared_lens[min(g0 + __ffsll(static_cast<long long>(here)) - 1, a.n_groups - 1)], 0);
         grouped = true;
       }
     }
     if (!grouped && cut == 0)       // nobody else tells of its shared keys
       for (int i = lane; i < G * a.cs; i += KVF_WAVE)
         t.ml[(static_cast<long>(seq) * a.H + kvh * G + i / a.cs) * (a.cs + a.co) + i % a.cs] = make_float2(-INFINITY, 0.f);
-    int hi = max(lo, min(t.ctx_lens[seq], most));
+    int hi = max(min(t.ctx_lens[seq], most), 0);
+    lo = min(lo, hi);
     cut_of(lo, hi, cut, a.co, BLOCK);
     for (int row0 = 0; row0 < G; row0 += 16) {
       Rows<T, DT, 1> x;
       x.start(t, a, seq, G, row0, kvh);
       x.template walk<ALIGNED>(t, a, t.table + static_cast<long>(seq) * a.width, kvh, lo & ~7, BLOCK, lo, hi);
-      x.leave(t, a, 0, x.m[0], x.whole_sum(0), seq, G, row0, kvh, a.cs + cut);
+      const long at = x.place(a, 0, seq, G, row0, kvh, a.cs + cut);
+      const float total = x.whole_sum(0);       // (all lanes take part)
+      if (x.leave_sum(t, 0, at, x.m[0], total, g == 0))
+#pragma unroll
+        for (int j = 0; j < DT; ++j)
+          if (j < a.d / 16) *reinterpret_cast<f32x4*>(t.acc + at * a.d + j * 16 + g * 4) = x.acc[0][j];
     }
   }
 }

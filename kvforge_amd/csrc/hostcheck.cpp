@@ -89,10 +89,56 @@ PyObject* operands(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
 }
 
+// Where a tensor's elements lie: [begin, end), empty for none.
+struct Span {
+  const char *begin, *end;
+};
+Span span_of(const at::Tensor& t) {
+  const char* at = static_cast<const char*>(t.const_data_ptr());
+  if (t.numel() == 0) return {at, at};
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  return {at, at + (last + 1) * static_cast<int64_t>(t.element_size())};
+}
+
+// placed(device, outs, ins): whether the tensors of both tuples (None is passed over) live on GPU number `device` and no span of
+// `outs` meets another tensor's.
+PyObject* placed(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  constexpr Py_ssize_t MOST = 16;
+  if (nargs != 3 || !PyLong_Check(args[0]) || !PyTuple_Check(args[1]) || !PyTuple_Check(args[2]) ||
+      PyTuple_GET_SIZE(args[1]) + PyTuple_GET_SIZE(args[2]) > MOST)
+    Py_RETURN_FALSE;
+  const long device = PyLong_AsLong(args[0]);
+  if (device == -1 && PyErr_Occurred()) PyErr_Clear();
+  try {
+    Span spans[MOST];
+    Py_ssize_t n = 0, outs = 0;
+    for (int side = 0; side < 2; ++side) {
+      PyObject* of = args[1 + side];
+      for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(of); ++i) {
+        PyObject* t = PyTuple_GET_ITEM(of, i);
+        if (t == Py_None) continue;
+        if (!THPVariable_Check(t)) Py_RETURN_FALSE;
+        const at::Tensor& x = THPVariable_Unpack(t);
+        if (!x.defined() || !x.is_cuda() || x.get_device() != device) Py_RETURN_FALSE;
+        spans[n++] = span_of(x);
+      }
+      if (side == 0) outs = n;
+    }
+    for (Py_ssize_t o = 0; o < outs; ++o)
+      for (Py_ssize_t i = o + 1; i < n; ++i)
+        if (spans[o].begin < spans[i].end && spans[i].begin < spans[o].end) Py_RETURN_FALSE;
+  } catch (...) {   // tensors without strides
+    Py_RETURN_FALSE;
+  }
+  Py_RETURN_TRUE;
+}
+
 PyMethodDef methods[] = {
     {"check", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(check)), METH_FASTCALL | METH_KEYWORDS, nullptr},
     {"set_slow", set_slow, METH_O, nullptr},
     {"operands", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(operands)), METH_FASTCALL, nullptr},
+    {"placed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(placed)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "hostcheck", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 }  // namespace

@@ -68,18 +68,27 @@ def _check(t: torch.Tensor, name: str, dtype=None, shape=None, contiguous=True) 
         raise KernelError(f"{name} must be contiguous")
 
 
-_check_in_python = _check
+def _placed(device: int, outs: tuple, ins: tuple) -> bool:
+    """Whether all tensors (``None`` is passed over) live on GPU number ``device`` and none of ``outs`` shares memory with
+    another."""
+    outs = [t for t in outs if t is not None]
+    tensors = outs + [t for t in ins if t is not None]
+    return (all(isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == device for t in tensors)
+            and not any(_overlap(o, t) for n, o in enumerate(outs) for t in tensors[n + 1:]))
+
+
+_check_in_python, _placed_in_python = _check, _placed
 _operands = None     # hostcheck's, once it is loaded
 
 
 def _check_natively() -> None:
     """From the first launch on operands are checked by native code, where there is any (``library.load_host``); what it does not
     pass goes to ``_check_in_python``, which says why."""
-    global _check, _operands
+    global _check, _operands, _placed
     native = library.load_host("hostcheck")
     if native is not None:
         native.set_slow(_check_in_python)
-        _check, _operands = native.check, native.operands
+        _check, _operands, _placed = native.check, native.operands, native.placed
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -1721,26 +1730,19 @@ def attn_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
 # ------------------------------------------------------------------------------ attention behind shared pages
 ATTN_BEAMS_MAX_CUTS = 64
 ATTN_BEAMS_KEYS_PER_CUT = 256
+_ATTN_BEAMS_ARGS = [c_int] + [c_void_p] * 11 + [c_int] * 13 + [c_float, c_void_p]
 
 
-def _here(who: str, first: torch.Tensor, *others) -> None:
-    """Launches go to the current device's stream: every operand lives there."""
-    at = first.get_device()
-    if at != torch.cuda.current_device():
-        raise KernelError(f"{who}: operands live on device {at}, the current one is {torch.cuda.current_device()}")
-    for t in others:
-        if t is not None and t.get_device() != at:
-            raise KernelError(f"{who}: operands live on several devices")
-
-
-def _apart(outs, ins) -> bool:
-    """Whether the memory of dense tensors ``outs`` lies apart from that of ``ins``, given as (address, bytes)."""
-    for o in outs:
-        a, b = o.data_ptr(), o.nbytes
-        for c, n in ins:
-            if a < c + n and c < a + b:
-                return False
-    return True
+def _here(who: str, outs: tuple, ins: tuple) -> int:
+    """The stream that a launch goes to, the current one of the current device: every operand lives there, and results lie apart
+    from what is read."""
+    device = torch.cuda.current_device()
+    if not _placed(device, outs, ins):
+        elsewhere = sorted({str(t.device) for t in (*outs, *ins) if t is not None and t.get_device() != device})
+        if elsewhere:
+            raise KernelError(f"{who}: the current device is {device}, operands live on {', '.join(elsewhere)}")
+        raise KernelError(f"{who}: results share memory with operands")
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
 def attn_beams_takes(dtype: torch.dtype, head_dim: int) -> bool:
@@ -1780,8 +1782,7 @@ def attn_beams(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     """Attention of one token per sequence (row ``i`` of ``q`` is sequence ``i``'s) over ``ctx_lens[i]`` cached keys, for
     sequences in groups ``cu_groups[g] .. cu_groups[g + 1] - 1`` whose first ``shared_lens[g]`` keys are the same, as the beams
     of a request have them behind its prompt: these are read once for the whole group, from the pages of its first
-    sequence that holds any.  (Of a group's sequences that hold keys, none may be shorter than what is shared; where one is, its length counts
-    as shared.)  A sequence without keys gets zeros; one that no group names shares nothing.  Page numbers outside the
+    sequence that holds any.  (One that is shorter than what its group shares attends over as many of the shared keys as it holds.)  A sequence without keys gets zeros; one that no group names shares nothing.  Page numbers outside the
     pages stand for keys that are not there.  ``widest``: sequences of the largest group (it decides how workgroups are laid out,
     results do not depend on it).  ``cuts`` from ``attn_beams_cuts``, ``workspace`` from ``attn_beams_workspace``; launches that
     share a workspace must not overlap.  ``sinks``: as in ``attn_prefill``.  Pages of any number of tokens (multiples of 8 are
@@ -1812,8 +1813,8 @@ def attn_beams(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     _check(shared_lens, "shared_lens", I32, (groups,))
     _check(ctx_lens, "ctx_lens", I32, (n,))
     _check(out, "out", q.dtype, (n, H * d))
-    if out.data_ptr() % 16 or (n and not _apart((out,), ((q.data_ptr(), ((n - 1) * q.stride(0) + H * d) * size),))):
-        raise KernelError("attn_beams: out starts on 16 bytes and does not share memory with q")
+    if out.data_ptr() % 16:
+        raise KernelError("attn_beams: out starts on 16 bytes")
     cs, co = int(cuts[0]), int(cuts[1])
     if not (0 <= cs <= ATTN_BEAMS_MAX_CUTS and 1 <= co <= ATTN_BEAMS_MAX_CUTS):
         raise KernelError(f"attn_beams: up to {ATTN_BEAMS_MAX_CUTS} cuts of the shared keys and 1 to {ATTN_BEAMS_MAX_CUTS} of a "
@@ -1828,11 +1829,11 @@ def attn_beams(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     if pa.shape[0] < n * H * (cs + co) * d or pm.shape[0] < n * H * (cs + co) * 2 or pa.data_ptr() % 16:
         raise KernelError("attn_beams: workspace too small")
     sk = _sinks_ptr(sinks, H, q)
-    _here("attn_beams", q, k_pages, v_pages, block_table, cu_groups, shared_lens, ctx_lens, out, pa, pm)
-    f = _fn("attn_beams", "kvf_attn_beams", [c_int] + [c_void_p] * 11 + [c_int] * 13 + [c_float, c_void_p])
+    stream = _here("attn_beams", (out, pa, pm), (q, k_pages, v_pages, block_table, cu_groups, shared_lens, ctx_lens, sinks))
+    f = _fn("attn_beams", "kvf_attn_beams", _ATTN_BEAMS_ARGS)
     _ok(f(_tcode(q.dtype), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), cu_groups.data_ptr(),
           shared_lens.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), pa.data_ptr(), pm.data_ptr(), sk, H, KV, d, bs, nb, width,
-          q.stride(0) if n > 1 else H * d, H * d, n, groups, int(widest), cs, co, float(scale), _stream()), "attn_beams")
+          q.stride(0) if n > 1 else H * d, H * d, n, groups, int(widest), cs, co, float(scale), stream), "attn_beams")
 
 
 # ------------------------------------------------------------------------------ matrix-memory recurrence
@@ -2895,6 +2896,7 @@ def decode_advance(sampled: torch.Tensor, token_ids: torch.Tensor, positions: to
 BEAM_MAX_COUNT = 64      # candidates of a request
 BEAM_MAX_WIDTH = 32      # beams of a request that are reordered together
 BEAM_PIECES = (2048, 8192)     # logits of a row that one workgroup takes
+_BEAM_REORDER_ARGS = [c_void_p] + [c_int] * 4 + [c_void_p] * 3
 _BEAM_SELECT_ARGS = [c_int, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 7
 
 
@@ -2942,11 +2944,6 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, cu_beams: torch.Tens
         raise KernelError(f"beam_select gives 1 to {BEAM_MAX_COUNT} candidates a request, asked for {count}")
     _check(out_beams, "out_beams", I32, (requests, count))
     _check(out_tokens, "out_tokens", I32, (requests, count))
-    stride = logits.stride(0) if rows > 1 else vocab
-    if rows and not _apart((out_scores, out_beams, out_tokens),
-                           ((logits.data_ptr(), ((rows - 1) * stride + vocab) * logits.element_size()),
-                            (scores.data_ptr(), 4 * rows), (cu_beams.data_ptr(), 4 * requests + 4))):
-        raise KernelError("beam_select: outputs do not share memory with inputs")
     pieces, piece = _beam_pieces(rows, vocab, count, logits.device)
     if pieces * count > 65536 or rows * pieces * count >= 2**31:
         raise KernelError(f"beam_select: {count} candidates of each of {pieces} pieces of {rows} rows are more than the kernel counts")
@@ -2956,11 +2953,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, cu_beams: torch.Tens
     _check(tokens, "workspace[2]", I32, (None,))
     if (sums.shape[0] < rows * pieces * 2 or min(values.shape[0], tokens.shape[0]) < rows * pieces * count or sums.data_ptr() % 16):
         raise KernelError("beam_select: workspace too small for these rows, logits and candidates")
-    _here("beam_select", logits, scores, cu_beams, out_scores, out_beams, out_tokens, *workspace)
+    stream = _here("beam_select", (out_scores, out_beams, out_tokens, sums, values, tokens), (logits, scores, cu_beams))
+    stride = logits.stride(0) if rows > 1 else vocab
     f = _fn("beam", "kvf_beam_select", _BEAM_SELECT_ARGS)
     _ok(f(_tcode(logits.dtype), logits.data_ptr(), stride, rows, vocab, scores.data_ptr(),
           cu_beams.data_ptr(), requests, count, pieces, piece, sums.data_ptr(), values.data_ptr(),
-          tokens.data_ptr(), out_scores.data_ptr(), out_beams.data_ptr(), out_tokens.data_ptr(), _stream()), "beam_select")
+          tokens.data_ptr(), out_scores.data_ptr(), out_beams.data_ptr(), out_tokens.data_ptr(), stream), "beam_select")
 
 
 class CacheRows:
@@ -3008,7 +3006,7 @@ def beam_reorder(rows: CacheRows, slots: torch.Tensor, parents: torch.Tensor) ->
     _check(parents, "parents", I32, (requests, beams))
     if not 1 <= beams <= BEAM_MAX_WIDTH or requests > 65535:
         raise KernelError(f"beam_reorder takes up to 65535 requests of 1 to {BEAM_MAX_WIDTH} beams, got {requests} of {beams}")
-    _here("beam_reorder", rows.tiles, slots, parents)
-    f = _fn("beam", "kvf_beam_reorder", [c_void_p] + [c_int] * 4 + [c_void_p] * 3)
+    stream = _here("beam_reorder", (), (rows.tiles, slots, parents))
+    f = _fn("beam", "kvf_beam_reorder", _BEAM_REORDER_ARGS)
     _ok(f(rows.tiles.data_ptr(), rows.tiles.shape[0], rows.rows, requests, beams, slots.data_ptr(),
-          parents.data_ptr(), _stream()), "beam_reorder")
+          parents.data_ptr(), stream), "beam_reorder")

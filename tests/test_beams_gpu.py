@@ -314,6 +314,11 @@ def test_shared_lengths_inside_a_page_and_beyond_a_sequence(dtype):
     few = [70, 20, 66] + ctx[3:]
     out = run_attend(q, k, v, same, cu, [64, 32], few, H, KV, d, 0.3)
     check_attend(out, q, k, v, same, few, H, KV, d, 0.3)
+    # the first of them the short one, with no more pages than it needs; nobody as long as what is said to be shared
+    short = [tables[0][:2] + [-1] * (len(tables[0]) - 2)] + [tables[0]] * 2 + tables[3:]
+    for few in ([20, 70, 66] + ctx[3:], [17, 30, 50] + ctx[3:], [0, 0, 40] + ctx[3:]):
+        out = run_attend(q, k, v, short, cu, [64, 32], few, H, KV, d, 0.3)
+        check_attend(out, q, k, v, short, few, H, KV, d, 0.3)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -120,3 +120,35 @@ def test_a_host_module_that_does_not_load_is_done_without(no_compiler, monkeypat
     broken.write_bytes(b"no library")
     monkeypatch.setattr(library, "_find_built", lambda name, want: str(broken))
     assert library.load_host("hostcheck") is None and len(no_compiler) == 1
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_native_placement_says_what_the_python_one_says(dev):
+    """Tensors beside each other, over each other, empty, with gaps, elsewhere, and what is no tensor."""
+    native = native_check()
+    one, two = torch.zeros(48, device=dev), torch.zeros(48, device=dev)
+    parts = [one, two, one[:16], one[16:32], one[15:17], one[:0], one.view(6, 8)[:, :3], one.view(6, 8)[:, 5:], one.view(6, 8)[1:, ::4], None, 5,
+             torch.zeros(3)]
+    said = set()
+    for a in parts:
+        for b in parts:
+            for c in (None, two):
+                for outs, ins in (((a,), (b, c)), ((a, b), (c,)), ((), (a, b, c)), ((a, c), ())):
+                    for device in (0, 1):
+                        got = native.placed(device, outs, ins)
+                        assert got == ops._placed_in_python(device, outs, ins), (device, outs, ins)
+                        said.add(got)
+    assert said == {True, False}
+    assert not native.placed(0, [one], ()) and not native.placed(0, (None,) * 9, (None,) * 9) and not native.placed(0, ())
+
+
+def test_results_that_share_memory_are_told_from_operands_elsewhere(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(ops, "_placed", ops._placed_in_python)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True, raising=False)
+    t = torch.zeros(8)
+    with pytest.raises(ops.KernelError, match="current device is 0, operands live on cpu"):
+        ops._here("op", (t,), ())
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    with pytest.raises(ops.KernelError, match="share memory"):
+        ops._here("op", (t[:4],), (t[3:],))

@@ -32,12 +32,16 @@ constexpr float LOG2E = 1.4426950408889634f;
 #define KVF_TWO_WAVES(FITS) __attribute__((amdgpu_waves_per_eu((FITS) ? 2 : 1)))
 
 struct Args {
-  int H, KV, d, bs, nb, width, q_stride, o_stride, n_seqs, n_groups;
+  int H, KV, G, d, bs, nb, width, q_stride, o_stride, n_seqs, n_groups;
   int blocks;          // row blocks of a group that have a workgroup of their own
   int cs, co;          // cuts of the shared keys and of a sequence's own
   float scale2;        // scale * log2(e)
+  float per_group;     // 1 / (H / KV)
   unsigned bs_magic;   // floor(2^32 / bs) + 1: key / bs == mulhi(key, bs_magic) while key * bs < 2^32
 };
+
+// row / G for rows below 2^22: (row + 0.5) / G lies no nearer to a whole number than 0.5 / G, which the roundings do not reach.
+__device__ __forceinline__ int group_of(int row, const Args& a) { return static_cast<int>((static_cast<float>(row) + 0.5f) * a.per_group); }
 
 __device__ __forceinline__ int page_of(int key, const Args& a) { return static_cast<int>(__umulhi(static_cast<unsigned>(key), a.bs_magic)); }
 
@@ -115,7 +119,9 @@ __device__ __forceinline__ int holder_of(int first, int n, int shared, const int
 }
 
 // What a wave holds of 16 * RT rows: Q, and the running reference, sum and accumulator of each.
-template <typename T, int DT, int RT> struct Rows {
+// FORM: WHOLE where d is 16 * DT and pages hold a multiple of 8 keys, ALIGNED where they do, ANY.
+enum Form { ANY, ALIGNED, WHOLE };
+template <typename T, int DT, int RT, Form FORM> struct Rows {
   typedef Frag<T> F;
   static constexpr int SLICES = DT * 16 / F::SLICE, LANE_D = F::SLICE / 4;
   typename F::Part q[RT][SLICES];
@@ -123,19 +129,25 @@ template <typename T, int DT, int RT> struct Rows {
   float m[RT], sum[RT];
   int ctx[RT];           // keys of the row's sequence
 
+  // A lane's part of a row from element e on, zeros behind the head's end (read inside it all the same).
+  static __device__ __forceinline__ bool has(int j, int tiles) { return FORM == WHOLE || j < tiles; }
+  static __device__ __forceinline__ typename F::Part part(const T* row, int e, int d) {
+    if constexpr (FORM == WHOLE) return F::load(row + e);
+    const typename F::Part v = F::load(row + min(e, d - LANE_D));
+    return e < d ? v : F::zero();
+  }
+
   // Rows [row0, row0 + 16 RT) of `rows`: sequence first + row / G, head row % G of kv head `kvh`.
   __device__ __forceinline__ void start(const Tensors<T>& t, const Args& a, int first, int rows, int row0, int kvh) {
-    const int lane = threadIdx.x % KVF_WAVE, g = lane / 16, r = lane % 16, G = a.H / a.KV;
+    const int lane = threadIdx.x % KVF_WAVE, g = lane / 16, r = lane % 16, G = a.G;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int row = min(row0 + rt * 16 + r, rows - 1);
-      ctx[rt] = t.ctx_lens[first + row / G];
-      const T* from = t.q + static_cast<long>(first + row / G) * a.q_stride + (kvh * G + row % G) * a.d;
+      const int seq = group_of(row, a);
+      ctx[rt] = t.ctx_lens[first + seq];
+      const T* from = t.q + static_cast<long>(first + seq) * a.q_stride + (kvh * G + row - seq * G) * a.d;
 #pragma unroll
-      for (int c = 0; c < SLICES; ++c) {
-        const int e = c * F::SLICE + g * LANE_D;
-        q[rt][c] = e < a.d ? F::load(from + e) : F::zero();
-      }
+      for (int c = 0; c < SLICES; ++c) q[rt][c] = part(from, c * F::SLICE + g * LANE_D, a.d);
       m[rt] = -INFINITY;
       sum[rt] = 0.f;
 #pragma unroll
@@ -145,10 +157,9 @@ template <typename T, int DT, int RT> struct Rows {
 
   // Blocks kb, kb + step, ... of the keys [lo, hi) of the pages in `table`.  kb: a multiple of 8.  The page numbers of a
   // block are looked up, and its K fragments loaded, while the block before it is worked on.
-  template <bool ALIGNED>
   __device__ __forceinline__ void walk(const Tensors<T>& t, const Args& a, const int* __restrict__ table, int kvh, int kb, int step, int lo, int hi) {
     const int lane = threadIdx.x % KVF_WAVE, g = lane / 16, r = lane % 16;
-    const int d = a.d, tiles = d / 16;
+    const int d = FORM == WHOLE ? DT * 16 : a.d, tiles = d / 16;
     const long page_elems = static_cast<long>(a.KV) * a.bs * d;
     const T* kp = t.k + static_cast<long>(kvh) * a.bs * d;
     const T* vp = t.v + static_cast<long>(kvh) * a.bs * d;
@@ -156,18 +167,15 @@ template <typename T, int DT, int RT> struct Rows {
     // the page that holds the keys from `key` on, -1 where there is none
     auto lookup = [&](int key) { return key < hi ? table[page_of(key, a)] : -1; };
     auto valid = [&](int page) { return page >= 0 && page < a.nb; };
-    auto load_k = [&](int at, int page) {         // ALIGNED: the page of keys at + 8 (r / 4)
-      if constexpr (ALIGNED) {
+    auto load_k = [&](int at, int page) {         // page (not for ANY): that of the keys at + 8 (r / 4)
+      if constexpr (FORM != ANY) {
         const int key = at + 8 * (r / 4);
         const bool ok = valid(page);
         const T* from = kp + (ok ? page : 0) * page_elems + static_cast<long>((ok ? key - page_of(key, a) * a.bs : 0) + r % 4) * d;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-          for (int c = 0; c < SLICES; ++c) {
-            const int e = c * F::SLICE + g * LANE_D;
-            kf[tt][c] = e < d ? F::load(from + tt * 4 * d + e) : F::zero();
-          }
+          for (int c = 0; c < SLICES; ++c) kf[tt][c] = part(from + tt * 4 * d, c * F::SLICE + g * LANE_D, d);
       } else {
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
@@ -175,16 +183,13 @@ template <typename T, int DT, int RT> struct Rows {
           const int p = key < hi ? table[key / a.bs] : -1;
           const T* from = kp + (valid(p) ? p : 0) * page_elems + static_cast<long>(valid(p) ? key % a.bs : 0) * d;
 #pragma unroll
-          for (int c = 0; c < SLICES; ++c) {
-            const int e = c * F::SLICE + g * LANE_D;
-            kf[tt][c] = e < d ? F::load(from + e) : F::zero();
-          }
+          for (int c = 0; c < SLICES; ++c) kf[tt][c] = part(from, c * F::SLICE + g * LANE_D, d);
         }
       }
     };
     if (kb >= hi) return;
-    int pv = 0;                          // ALIGNED: the page of keys kb + 8 g
-    if constexpr (ALIGNED) {
+    int pv = 0;                          // (not for ANY) the page of keys kb + 8 g
+    if constexpr (FORM != ANY) {
       const int pk = lookup(kb + 8 * (r / 4));
       pv = lookup(kb + 8 * g);
       load_k(kb, pk);
@@ -196,14 +201,14 @@ template <typename T, int DT, int RT> struct Rows {
       typename F::Keys vf[DT];
       unsigned keep = 0;                // which of the lane's keys kb + 8 g + (0 .. 7) count
       int pk_next = -1, pv_next = -1;
-      if constexpr (ALIGNED) {
+      if constexpr (FORM != ANY) {
         const int key = kb + 8 * g, from = max(lo - key, 0), to = min(hi - key, 8);
         const bool ok = valid(pv);
         keep = ok && to > from ? (0xffu >> (8 - to)) & (0xffu << from) : 0u;
         const T* v0 = vp + (ok ? pv : 0) * page_elems + (ok ? key - page_of(key, a) * a.bs : 0) + r * a.bs;
 #pragma unroll
         for (int j = 0; j < DT; ++j)
-          if (j < tiles) vf[j] = F::load_keys(v0 + static_cast<long>(j) * 16 * a.bs);
+          if (has(j, tiles)) vf[j] = F::load_keys(v0 + static_cast<long>(j) * 16 * a.bs);
         pk_next = lookup(next + 8 * (r / 4));
         pv_next = lookup(next + 8 * g);
       } else {
@@ -215,7 +220,7 @@ template <typename T, int DT, int RT> struct Rows {
           const T* v0 = vp + (valid(p) ? p : 0) * page_elems + (valid(p) ? key % a.bs : 0) + r * a.bs;
 #pragma unroll
           for (int j = 0; j < DT; ++j)
-            if (j < tiles) F::set(vf[j], i, v0[static_cast<long>(j) * 16 * a.bs]);
+            if (has(j, tiles)) F::set(vf[j], i, v0[static_cast<long>(j) * 16 * a.bs]);
         }
       }
       const bool whole = __all(keep == 0xffu);
@@ -268,23 +273,22 @@ template <typename T, int DT, int RT> struct Rows {
       if (!whole)
 #pragma unroll
         for (int j = 0; j < DT; ++j)
-          if (j < tiles) F::clear(vf[j], keep);
+          if (has(j, tiles)) F::clear(vf[j], keep);
 #pragma unroll
       for (int j = 0; j < DT; ++j)
-        if (j < tiles)
+        if (has(j, tiles))
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) acc[rt][j] = F::values(vf[j], pf[rt], acc[rt][j]);
       if (next >= hi) break;
       kb = next;
       pv = pv_next;
-      if constexpr (!ALIGNED) (void)pk_next;
     }
   }
 
   // Where row rt * 16 + r of the rows leaves its results as cut `cut`; -1: nowhere.
   __device__ __forceinline__ long place(const Args& a, int rt, int first, int rows, int row0, int kvh, int cut) const {
-    const int r = threadIdx.x % 16, G = a.H / a.KV, row = row0 + rt * 16 + r;
-    return row < rows ? (static_cast<long>(first + row / G) * a.H + kvh * G + row % G) * (a.cs + a.co) + cut : -1;
+    const int r = threadIdx.x % 16, G = a.G, row = row0 + rt * 16 + r, seq = group_of(row, a);
+    return row < rows ? (static_cast<long>(first + seq) * a.H + kvh * G + row - seq * G) * (a.cs + a.co) + cut : -1;
   }
   // (reference, sum over all keys of the cut), -inf where there are none (NaN stays NaN); whether there is an accumulator.
   __device__ __forceinline__ bool leave_sum(const Tensors<T>& t, int rt, long at, float top, float total, bool writes) const {
@@ -311,12 +315,12 @@ __device__ __forceinline__ void cut_of(int& lo, int& hi, int c, int n, int round
 // The workgroups of the first n_groups * cs * blocks * KV numbers take a cut of a group's shared keys, the four waves a block
 // each in turn; of the others every wave takes a cut of a sequence's own keys by itself.  The kv head is the fastest index:
 // workgroups go to the eight XCDs in turn, so with eight heads an L2 holds the keys of one, also for a group's further rows.
-template <typename T, int DT, int RT, bool ALIGNED>
+template <typename T, int DT, int RT, Form FORM>
 __global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 16 && DT < 16 : RT * DT <= 8) void attn_beams_kernel(Tensors<T> t, Args a) {
   __shared__ f32x4 lds_acc[RT][DT][WAVES - 1][KVF_WAVE];
   __shared__ float2 lds_ml[RT][WAVES][16];
   const int shared_items = a.n_groups * a.cs * a.blocks * a.KV;
-  const int G = a.H / a.KV, most = a.width * a.bs, lane = threadIdx.x % KVF_WAVE, wave = threadIdx.x / KVF_WAVE, g = lane / 16, r = lane % 16;
+  const int G = a.G, most = a.width * a.bs, lane = threadIdx.x % KVF_WAVE, wave = threadIdx.x / KVF_WAVE, g = lane / 16, r = lane % 16;
   if (static_cast<int>(blockIdx.x) < shared_items) {
     const int item = blockIdx.x;
     const int kvh = item % a.KV, block = item / a.KV % a.blocks, cut = item / a.KV / a.blocks % a.cs, group = item / a.KV / a.blocks / a.cs;
@@ -327,9 +331,10 @@ __global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 
     const int holder = holder_of(first, n, hi, t.ctx_lens);
     cut_of(lo, hi, cut, a.cs, WAVES * BLOCK);
     for (int row0 = block * 16 * RT; row0 < rows; row0 += a.blocks * 16 * RT) {
-      Rows<T, DT, RT> x;
+      typedef Rows<T, DT, RT, FORM> Held;
+      Held x;
       x.start(t, a, first, rows, row0, kvh);
-      x.template walk<ALIGNED>(t, a, t.table + static_cast<long>(holder) * a.width, kvh, lo + wave * BLOCK, WAVES * BLOCK, lo, hi);
+      x.walk(t, a, t.table + static_cast<long>(holder) * a.width, kvh, lo + wave * BLOCK, WAVES * BLOCK, lo, hi);
       // the waves' results: tile j of the elements is summed by wave j % WAVES
       float l[RT];
 #pragma unroll
@@ -356,7 +361,7 @@ __global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 
 #pragma unroll
         for (int j = 0; j < DT; ++j) {
           x.acc[rt][j] *= by;
-          if (j % WAVES != wave && j < tiles) lds_acc[rt][j][wave < j % WAVES ? wave : wave - 1][lane] = x.acc[rt][j];
+          if (j % WAVES != wave && Held::has(j, tiles)) lds_acc[rt][j][wave < j % WAVES ? wave : wave - 1][lane] = x.acc[rt][j];
         }
       }
       __syncthreads();
@@ -364,7 +369,7 @@ __global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int j = 0; j < DT; ++j)
-          if (j % WAVES == wave && j < tiles) {
+          if (j % WAVES == wave && Held::has(j, tiles)) {
             f32x4 o = x.acc[rt][j];
 #pragma unroll
             for (int w = 0; w < WAVES - 1; ++w) o += lds_acc[rt][j][w][lane];
@@ -394,63 +399,92 @@ __global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 
     lo = min(lo, hi);
     cut_of(lo, hi, cut, a.co, BLOCK);
     for (int row0 = 0; row0 < G; row0 += 16) {
-      Rows<T, DT, 1> x;
+      typedef Rows<T, DT, 1, FORM> Held;
+      Held x;
       x.start(t, a, seq, G, row0, kvh);
-      x.template walk<ALIGNED>(t, a, t.table + static_cast<long>(seq) * a.width, kvh, lo & ~7, BLOCK, lo, hi);
+      x.walk(t, a, t.table + static_cast<long>(seq) * a.width, kvh, lo & ~7, BLOCK, lo, hi);
       const long at = x.place(a, 0, seq, G, row0, kvh, a.cs + cut);
       const float total = x.whole_sum(0);       // (all lanes take part)
       if (x.leave_sum(t, 0, at, x.m[0], total, g == 0))
 #pragma unroll
         for (int j = 0; j < DT; ++j)
-          if (j < a.d / 16) *reinterpret_cast<f32x4*>(t.acc + at * a.d + j * 16 + g * 4) = x.acc[0][j];
+          if (Held::has(j, a.d / 16)) *reinterpret_cast<f32x4*>(t.acc + at * a.d + j * 16 + g * 4) = x.acc[0][j];
     }
   }
 }
 
-// A wave a row: the cuts' sums and accumulators at the largest of their references.  Lanes: four elements each, of up to four cuts
+__device__ __forceinline__ float wave_of(float v, bool sum) {
+  auto with = [&](float other) { v = sum ? v + other : fmaxf(v, other); };
+  with(dpp_move<0xB1>(v));        // lane ^ 1
+  with(dpp_move<0x4E>(v));        // lane ^ 2
+  with(dpp_move<0x141>(v));       // the other four of 8 lanes
+  with(dpp_move<0x140>(v));       // the other eight of 16
+  with(__shfl_xor(v, 16, KVF_WAVE));
+  with(__shfl_xor(v, 32, KVF_WAVE));
+  return v;
+}
+
+// The cuts' sums and accumulators of a row at the largest of their references.  A wave takes a row, or with PARTS waves each
+// every so many of its cuts (32 cuts of 256 rows: 6.4 us a wave a row, 4.6 four).  Lanes: four elements each, of up to four cuts
 // side by side.
-template <typename T>
-__global__ __launch_bounds__(THREADS) void attn_beams_join_kernel(const float* __restrict__ acc, const float2* __restrict__ ml,
-                                                                  T* __restrict__ out, const float* __restrict__ sinks, Args a) {
-  const int lane = threadIdx.x % KVF_WAVE, cuts = a.cs + a.co;
-  const long row = static_cast<long>(blockIdx.x) * WAVES + threadIdx.x / KVF_WAVE;
-  if (row >= static_cast<long>(a.n_seqs) * a.H) return;
+template <typename T, int PARTS>
+__global__ __launch_bounds__(THREADS) void attn_beams_join_kernel(const float* acc, const float2* ml, T* __restrict__ out,
+                                                                  const float* sinks, Args a) {
+  __shared__ f32x4 lds[WAVES][KVF_WAVE];
+  const int lane = threadIdx.x % KVF_WAVE, wave = threadIdx.x / KVF_WAVE, cuts = a.cs + a.co;
+  const int part = wave % PARTS;
+  const long last = static_cast<long>(a.n_seqs) * a.H - 1, want = static_cast<long>(blockIdx.x) * (WAVES / PARTS) + wave / PARTS;
+  if (PARTS == 1 && want > last) return;
+  const long row = want;       // (PARTS > 1: as many workgroups as rows)
   const int h = static_cast<int>(row % a.H);
   const float2* mine = ml + row * cuts;
-  float top = -INFINITY;
-  for (int c = lane; c < cuts; c += KVF_WAVE) top = fmaxf(top, mine[c].x);
-  top = wave_max(top);
-  const bool any = top > -INFINITY;
-  if (sinks != nullptr) top = fmaxf(top, sinks[h] * LOG2E);
-  float total = 0.f;
-  for (int c = lane; c < cuts; c += KVF_WAVE)
-    if (mine[c].x > -INFINITY) total += mine[c].y * __builtin_amdgcn_exp2f(mine[c].x - top);
-  total = wave_sum(total);
-  if (sinks != nullptr) total += __builtin_amdgcn_exp2f(sinks[h] * LOG2E - top);
   const int quads = a.d / 4, side = quads > 32 ? 1 : quads > 16 ? 2 : 4;
   const int sub = lane / (KVF_WAVE / side), at = lane % (KVF_WAVE / side);
-  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (at < quads) {
-    // four cuts in flight; one without keys has left no accumulator: what is read in its place is not used
-    constexpr int U = 4;
-    const float* from = acc + row * cuts * a.d + at * 4;
-    for (int c0 = sub; c0 < cuts; c0 += U * side) {
-      f32x4 v[U];
-      float2 x[U];
+  // accumulators of U cuts in flight, the first ahead of everything else; one without keys has left none: what is read in its
+  // place is not used
+  constexpr int U = 4;
+  const int step = side * PARTS;
+  const float* from = acc + row * cuts * a.d + min(at, quads - 1) * 4;
+  f32x4 v[U];
+  float2 x[U];
+  auto load = [&](int c0) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int c = min(c0 + u * side, cuts - 1);
-        x[u] = mine[c];
-        v[u] = *reinterpret_cast<const f32x4*>(from + static_cast<long>(c) * a.d);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (c0 + u * side < cuts && x[u].x > -INFINITY) o += v[u] * __builtin_amdgcn_exp2f(x[u].x - top);
+    for (int u = 0; u < U; ++u) {
+      const int c = min(c0 + u * step, cuts - 1);
+      x[u] = mine[c];
+      v[u] = *reinterpret_cast<const f32x4*>(from + static_cast<long>(c) * a.d);
     }
+  };
+  const int first = sub * PARTS + part;
+  load(first);
+  const float2 none = make_float2(-INFINITY, 0.f);
+  const float2 one = lane < cuts ? mine[lane] : none, two = lane + KVF_WAVE < cuts ? mine[lane + KVF_WAVE] : none;
+  const float sink = sinks != nullptr ? sinks[h] * LOG2E : -INFINITY;
+  float top = wave_of(fmaxf(one.x, two.x), false);
+  const bool any = top > -INFINITY;
+  top = fmaxf(top, sink);
+  const float ref = top > -INFINITY ? top : 0.f;
+  auto weight = [&](float m) { return __builtin_amdgcn_exp2f(m - ref); };      // 0 of -inf
+  float total = (one.x > -INFINITY ? one.y * weight(one.x) : 0.f) + (two.x > -INFINITY ? two.y * weight(two.x) : 0.f);
+  total = wave_of(total, true) + weight(sink);
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int c0 = first; c0 < cuts; c0 += U * step) {
+    if (c0 != first) load(c0);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * step < cuts && x[u].x > -INFINITY) o += v[u] * weight(x[u].x);
   }
   for (int s = KVF_WAVE / side; s < KVF_WAVE; s *= 2)
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], s, KVF_WAVE);
+  if constexpr (PARTS > 1) {
+    static_assert(PARTS == WAVES, "a row a workgroup");
+    lds[wave][lane] = o;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) o += lds[w][lane];
+  }
   if (sub == 0 && at < quads) {
     T* to = out + row / a.H * a.o_stride + static_cast<long>(h) * a.d + at * 4;
 #pragma unroll
@@ -462,43 +496,59 @@ __global__ __launch_bounds__(THREADS) void attn_beams_join_kernel(const float* _
 template <typename T> constexpr int TWO_TILES = sizeof(T) == 2 ? 128 : 64;
 int row_tiles_of(int bf16, int d, int bs, int rows) { return rows > 16 && d <= (bf16 ? TWO_TILES<bf16_t> : TWO_TILES<float>) && bs % 8 == 0 ? 2 : 1; }
 
-template <typename T, int DT, bool ALIGNED>
-int launch_rows(const Tensors<T>& t, const Args& a, int row_tiles, hipStream_t stream) {
+template <typename T, int DT, int RT, Form FORM>
+int launch(const Tensors<T>& t, const Args& a, int* per_cu, hipStream_t stream) {
+  if (per_cu)      // asked how many workgroups a compute unit holds
+    return static_cast<int>(hipOccupancyMaxActiveBlocksPerMultiprocessor(per_cu, attn_beams_kernel<T, DT, RT, FORM>, THREADS, 0));
   const long items = static_cast<long>(a.n_groups) * a.cs * a.blocks * a.KV + (static_cast<long>(a.n_seqs) * a.co * a.KV + WAVES - 1) / WAVES;
   if (items * WAVES > 0x7fffffffL) return static_cast<int>(hipErrorInvalidValue);
-  const dim3 grid(static_cast<unsigned>(items));
-  if constexpr (ALIGNED && DT <= TWO_TILES<T> / 16) {
-    if (row_tiles == 2) {
-      attn_beams_kernel<T, DT, 2, ALIGNED><<<grid, THREADS, 0, stream>>>(t, a);
-      return kvf_last_error();
-    }
-  }
-  attn_beams_kernel<T, DT, 1, ALIGNED><<<grid, THREADS, 0, stream>>>(t, a);
+  attn_beams_kernel<T, DT, RT, FORM><<<dim3(static_cast<unsigned>(items)), THREADS, 0, stream>>>(t, a);
   return kvf_last_error();
 }
-template <typename T, bool ALIGNED>
-int launch_dims(const Tensors<T>& t, const Args& a, int row_tiles, hipStream_t stream) {
-  if (a.d <= 32) return launch_rows<T, 2, ALIGNED>(t, a, row_tiles, stream);
-  if (a.d <= 64) return launch_rows<T, 4, ALIGNED>(t, a, row_tiles, stream);
-  if (a.d <= 96) return launch_rows<T, 6, ALIGNED>(t, a, row_tiles, stream);
-  if (a.d <= 128) return launch_rows<T, 8, ALIGNED>(t, a, row_tiles, stream);
-  return launch_rows<T, 16, ALIGNED>(t, a, row_tiles, stream);
+template <typename T, int DT> int launch_form(const Tensors<T>& t, const Args& a, int row_tiles, int* per_cu, hipStream_t stream) {
+  if (a.bs % 8) return launch<T, DT, 1, ANY>(t, a, per_cu, stream);
+  if constexpr (DT <= TWO_TILES<T> / 16)
+    if (row_tiles == 2) return a.d == DT * 16 ? launch<T, DT, 2, WHOLE>(t, a, per_cu, stream) : launch<T, DT, 2, ALIGNED>(t, a, per_cu, stream);
+  return a.d == DT * 16 ? launch<T, DT, 1, WHOLE>(t, a, per_cu, stream) : launch<T, DT, 1, ALIGNED>(t, a, per_cu, stream);
 }
+template <typename T> int launch_dims(const Tensors<T>& t, const Args& a, int row_tiles, int* per_cu, hipStream_t stream) {
+  if (a.d <= 32) return launch_form<T, 2>(t, a, row_tiles, per_cu, stream);
+  if (a.d <= 64) return launch_form<T, 4>(t, a, row_tiles, per_cu, stream);
+  if (a.d <= 96) return launch_form<T, 6>(t, a, row_tiles, per_cu, stream);
+  if (a.d <= 128) return launch_form<T, 8>(t, a, row_tiles, per_cu, stream);
+  return launch_form<T, 16>(t, a, row_tiles, per_cu, stream);
+}
+constexpr int JOIN_WIDE = 16;     // more cuts of a row than so many are joined by four waves
+
 template <typename T>
 int run(const void* q, const void* k, const void* v, const int* table, const int* cu_groups, const int* shared_lens, const int* ctx_lens,
         void* out, float* acc, void* ml, const float* sinks, const Args& a, int row_tiles, hipStream_t stream) {
   const Tensors<T> t{static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), table, cu_groups, shared_lens, ctx_lens,
                      acc, static_cast<float2*>(ml)};
-  const int rc = a.bs % 8 == 0 ? launch_dims<T, true>(t, a, row_tiles, stream) : launch_dims<T, false>(t, a, row_tiles, stream);
+  const int rc = launch_dims<T>(t, a, row_tiles, nullptr, stream);
   if (rc) return rc;
   const long rows = static_cast<long>(a.n_seqs) * a.H;
-  attn_beams_join_kernel<T><<<static_cast<unsigned>((rows + WAVES - 1) / WAVES), THREADS, 0, stream>>>(acc, static_cast<const float2*>(ml), static_cast<T*>(out), sinks, a);
+  if (a.cs + a.co > JOIN_WIDE && rows <= 0x7fffffffL / THREADS)
+    attn_beams_join_kernel<T, WAVES><<<static_cast<unsigned>(rows), THREADS, 0, stream>>>(acc, static_cast<const float2*>(ml), static_cast<T*>(out), sinks, a);
+  else
+    attn_beams_join_kernel<T, 1><<<static_cast<unsigned>((rows + WAVES - 1) / WAVES), THREADS, 0, stream>>>(acc, static_cast<const float2*>(ml), static_cast<T*>(out), sinks, a);
   return kvf_last_error();
 }
 }  // namespace
 
 // Tiles of 16 rows that a workgroup takes where a group has `rows` rows a kv head.
 KVF_EXPORT int kvf_attn_beams_row_tiles(int bf16, int d, int bs, int rows) { return row_tiles_of(bf16, d, bs, rows); }
+
+// Workgroups that a compute unit holds of the kernel that such heads take (0: it cannot be said).
+KVF_EXPORT int kvf_attn_beams_blocks_per_cu(int bf16, int d, int bs, int rows) {
+  if (d < 16 || d > 256 || d % 16 || bs < 1) return 0;
+  Args a{};
+  a.d = d;
+  a.bs = bs;
+  int n = 0;
+  const int rc = bf16 ? launch_dims<bf16_t>({}, a, row_tiles_of(1, d, bs, rows), &n, nullptr) : launch_dims<float>({}, a, row_tiles_of(0, d, bs, rows), &n, nullptr);
+  return rc ? 0 : n;
+}
 
 // q [n_seqs] rows of H heads; pages k [nb, KV, bs, d], v [nb, KV, d, bs]; table [n_seqs, width]; cu_groups [n_groups + 1];
 // shared_lens [n_groups]; ctx_lens [n_seqs].  Workspace: acc [n_seqs, H, cs + co, d], ml [n_seqs, H, cs + co, 2].
@@ -514,7 +564,7 @@ KVF_EXPORT int kvf_attn_beams(int bf16, const void* q, const void* k, const void
   const long rows = static_cast<long>(widest) * (H / KV);
   if (rows > 1 << 20) return static_cast<int>(hipErrorInvalidValue);
   const int row_tiles = row_tiles_of(bf16, d, bs, static_cast<int>(rows)), blocks = static_cast<int>((rows + 16 * row_tiles - 1) / (16 * row_tiles));
-  const Args a{H, KV, d, bs, nb, width, q_stride, o_stride, n_seqs, n_groups, blocks, cs, co, scale * LOG2E,
+  const Args a{H, KV, H / KV, d, bs, nb, width, q_stride, o_stride, n_seqs, n_groups, blocks, cs, co, scale * LOG2E, 1.f / static_cast<float>(H / KV),
                bs > 1 ? static_cast<unsigned>((1ull << 32) / bs) + 1u : 0u};
   return bf16 ? run<bf16_t>(q, k, v, table, cu_groups, shared_lens, ctx_lens, out, acc, ml, sinks, a, row_tiles, stream)
               : run<float>(q, k, v, table, cu_groups, shared_lens, ctx_lens, out, acc, ml, sinks, a, row_tiles, stream);

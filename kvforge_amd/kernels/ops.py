@@ -1729,7 +1729,8 @@ def attn_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
 
 # ------------------------------------------------------------------------------ attention behind shared pages
 ATTN_BEAMS_MAX_CUTS = 64
-ATTN_BEAMS_KEYS_PER_CUT = 256
+ATTN_BEAMS_ROUND = 128       # keys that the waves of a workgroup take at a time
+ATTN_BEAMS_OWN_KEYS = 64     # keys of a sequence's own that are worth a wave
 _ATTN_BEAMS_ARGS = [c_int] + [c_void_p] * 11 + [c_int] * 13 + [c_float, c_void_p]
 
 
@@ -1750,22 +1751,35 @@ def attn_beams_takes(dtype: torch.dtype, head_dim: int) -> bool:
     return dtype in (F32, BF16) and 0 < head_dim <= 256 and head_dim % 16 == 0
 
 
+@lru_cache(maxsize=None)
+def _attn_beams_held(bf16: int, head_dim: int, block_size: int, rows: int) -> tuple[int, int]:
+    """(tiles of 16 rows a workgroup takes, workgroups a compute unit holds) of the kernel for groups of ``rows`` rows a kv head."""
+    tiles = _fn("attn_beams", "kvf_attn_beams_row_tiles", [c_int] * 4)(bf16, head_dim, block_size, rows)
+    held = _fn("attn_beams", "kvf_attn_beams_blocks_per_cu", [c_int] * 4)(bf16, head_dim, block_size, rows)
+    return int(tiles), int(held) or 2
+
+
 def attn_beams_cuts(q: torch.Tensor, k_pages: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, num_groups: int,
                     num_seqs: int, widest: int, max_shared: int, max_own: int) -> tuple[int, int]:
-    """(cuts of the keys that a group shares, cuts of a sequence's own keys) for ``attn_beams``: two workgroups a compute unit
-    over the shared keys and 16 waves over the others, where the keys suffice for cuts of ``ATTN_BEAMS_KEYS_PER_CUT`` and a quarter
-    of it.  ``max_shared``, ``max_own``: the most shared keys of a group and own keys of a sequence (any cuts give right
-    results for any lengths)."""
+    """(cuts of the keys that a group shares, cuts of a sequence's own keys) for ``attn_beams``.  Own keys: up to eight waves a
+    compute unit, each with ``ATTN_BEAMS_OWN_KEYS``.  Shared ones: as many workgroups as the chip holds beside those of the
+    own keys, for what does not find room at once starts only when others end (2 x 8,192 shared keys of 4 beams, heads of 128:
+    12 cuts 20.0 us, 30 that fit 18.8, 32 that do not 22.2), each with a round of its waves at least (two in fp32).
+    ``max_shared``, ``max_own``: the most shared keys of a group and own keys of a sequence (any cuts give right results for
+    any lengths)."""
     units = compute_units(q.device)
     rows = max(1, widest) * (num_heads // num_kv_heads)
-    tiles = int(_fn("attn_beams", "kvf_attn_beams_row_tiles", [c_int] * 4)(_tcode(q.dtype), head_dim, k_pages.shape[2], rows))
-    shared = num_groups * num_kv_heads * -(-rows // (16 * tiles))
+    tiles, held = _attn_beams_held(_tcode(q.dtype), head_dim, k_pages.shape[2], rows)
 
-    def cuts(room: int, groups: int, keys: int, per: int) -> int:
-        return max(1, min(-(-room // max(groups, 1)), -(-keys // per), ATTN_BEAMS_MAX_CUTS))
+    def cuts(room: int, items: int, keys: int, per: int) -> int:
+        return max(1, min(room // max(items, 1), -(-keys // per), ATTN_BEAMS_MAX_CUTS))
 
-    return (cuts(2 * units, shared, max_shared, ATTN_BEAMS_KEYS_PER_CUT) if num_groups and max_shared > 0 else 0,
-            cuts(16 * units, num_seqs * num_kv_heads, max_own, ATTN_BEAMS_KEYS_PER_CUT // 4))
+    own = cuts(8 * units, num_seqs * num_kv_heads, max_own, ATTN_BEAMS_OWN_KEYS)
+    if not num_groups or max_shared <= 0:
+        return 0, own
+    room = held * units - -(-num_seqs * num_kv_heads * own // 4)
+    return cuts(room, num_groups * num_kv_heads * -(-rows // (16 * tiles)), max_shared,
+                ATTN_BEAMS_ROUND if q.dtype == BF16 else 2 * ATTN_BEAMS_ROUND), own
 
 
 def attn_beams_workspace(num_seqs: int, num_heads: int, head_dim: int, cuts: tuple[int, int], device

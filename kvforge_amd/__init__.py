@@ -19,6 +19,9 @@ __version__ = "0.1.0"
 _LAZY = {
     "InferenceEngine": "kvforge_amd.engine.engine",
     "SamplingParams": "kvforge_amd.sampling.params",
+    "BeamParams": "kvforge_amd.sampling.params",
+    "BeamOutput": "kvforge_amd.engine.beams",
+    "BeamSequence": "kvforge_amd.engine.beams",
     "Request": "kvforge_amd.engine.request",
     "RequestOutput": "kvforge_amd.engine.request",
     "RequestStatus": "kvforge_amd.engine.request",

@@ -203,6 +203,56 @@ class CacheManager:
         if total_tokens > self._num_tokens[request_id]:
             self._num_tokens[request_id] = total_tokens
 
+    def branch(self, request_id: str, parent_id: str, num_tokens: int) -> None:
+        """``request_id`` goes on from ``parent_id``'s first ``num_tokens`` positions, all that the parent's tables hold: it
+        shares the pages that these fill and gets one of its own, per group, for the page that they begin to fill (whose
+        contents the caller copies: the last entry of the parent's table into the last of this one's).  What it held before is
+        given back.  Raises before anything changes if a pool is short."""
+        if request_id == parent_id:
+            raise ValueError(f"request {request_id} cannot go on from itself")
+        if self._num_tokens[parent_id] < num_tokens:
+            raise ValueError(f"request {parent_id} holds {self._num_tokens[parent_id]} tokens, not {num_tokens}")
+        whole, need = num_tokens // self.block_size, self.blocks_needed(num_tokens)
+        known = request_id in self._num_tokens
+        for g, p in enumerate(self.pools):
+            if len(self._tables[g][parent_id]) != need:
+                raise ValueError(f"the tables of {parent_id} hold more or fewer pages than {num_tokens} tokens need")
+            own = sum(b != RELEASED and p.ref_count(b) == 1 for b in self._tables[g][request_id]) if known else 0
+            if need - whole > p.num_free + own:
+                raise NoFreeBlocksError(f"no page for {request_id} to go on from {parent_id}")
+        if self.slots.num_slots and not self.slots.has(request_id):
+            self.slots.take(request_id)
+        for g, p in enumerate(self.pools):
+            table = self._tables[g][parent_id][:whole]
+            for b in table:
+                if b != RELEASED:
+                    p.share(b)
+            for b in reversed(self._tables[g].get(request_id, ())):
+                if b != RELEASED:
+                    p.release(b)
+            if need > whole:
+                table.append(p.take())
+            self._tables[g][request_id] = table
+            self._released[g][request_id] = self._released[g][parent_id]
+        self._num_tokens[request_id] = num_tokens
+        self._serial[request_id] = self._next_serial
+        self._next_serial += 1
+
+    def shared_pages(self, request_ids: "list[str]", known: int = 0) -> int:
+        """How many entries at the start of the requests' tables are the same in all of them and every group without a window
+        (``known``: so many are)."""
+        n = None
+        for g, group in enumerate(self.groups):
+            if group.window is not None:
+                continue
+            tables = [self._tables[g][r] for r in request_ids]
+            most = min(map(len, tables))
+            i = min(known, most)
+            while i < most and all(t[i] == tables[0][i] for t in tables):
+                i += 1
+            n = i if n is None else min(n, i)
+        return n or 0
+
     def release_behind(self, request_id: str, num_computed: int) -> int:
         """Give back pages of windowed groups that no later query can see: the next query sits at
         position ``num_computed`` and sees keys from ``num_computed - window + 1`` on.  Returns

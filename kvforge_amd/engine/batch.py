@@ -28,6 +28,31 @@ class DecodeShape:
     n: int
     max_ctx: int
     sum_ctx: int
+    groups: "SharedShape | None" = None      # sequences that share pages, if the step says so (``SharedPages``)
+
+
+@dataclass(frozen=True)
+class SharedShape:
+    """Groups of sequences that share their first pages, as far as launches depend on them: how many groups, the sequences of
+    the largest, and the most shared keys of a group and own keys of a sequence, both rounded up to whole cells."""
+
+    groups: int
+    widest: int
+    max_shared: int
+    max_own: int
+
+    SHARED_CELL = 512
+    OWN_CELL = 64
+
+
+@dataclass
+class SharedPages:
+    """A step's groups on the device: ``cu_groups`` (group ``g`` is the sequences ``cu_groups[g] .. cu_groups[g + 1] - 1``) and the
+    keys that each shares; what the launches depend on."""
+
+    cu_groups: torch.Tensor
+    shared_lens: torch.Tensor
+    shape: SharedShape
 
 
 @dataclass
@@ -141,7 +166,7 @@ class MetaBuffers:
         self.off: dict[str, int] = {}
         # ("run_counter" is zero in the staging memory: every batch that is sent begins a run's count anew)
         for name, size in (("run_counter", 1), ("cu_q", max_seqs + 1), ("ctx_lens", max_seqs), ("slot_ids", max_seqs),
-                           ("decode_seq_ids", max_seqs), ("token_ids", max_tokens),
+                           ("cu_groups", max_seqs + 1), ("shared_lens", max_seqs), ("decode_seq_ids", max_seqs), ("token_ids", max_tokens),
                            ("positions", max_tokens), ("seq_of_token", max_tokens),
                            ("logits_rows", max_tokens)):
             self.off[name] = off
@@ -211,6 +236,7 @@ class Step:
         self.host_token_ids: np.ndarray | None = None
         self.prefill_seqs: list[int] = []
         self.decode_shape = DecodeShape(0, 0, 0)
+        self.shared: SharedPages | None = None
         self.all_rows = False        # every token wants its logits, in order
         self.max_position = 0
         # What parts keep for the length of the step (work lists, launch plans, tables), under
@@ -473,7 +499,7 @@ def extend_tables(meta: "MetaBuffers", entries: Sequence[StepEntry], padded: int
 def fill_step(step: Step, meta: MetaBuffers, entries: Sequence[StepEntry], tables_of, slot_of,
               block_size: int, pad_to: int | None = None,
               windowed_groups: Sequence[bool] | None = None, serial_of=None,
-              lookahead: int = 0) -> list[int]:
+              lookahead: int = 0, shared: "Sequence[tuple[int, int]] | None" = None) -> list[int]:
     """Write the batch into ``meta`` (one host-to-device copy) and point ``step`` at it.
     ``tables_of(request_id, group) -> list[int]``; ``slot_of(request_id) -> int``.
     ``pad_to``: pad a pure-decode batch with empty sequences up to this many.
@@ -482,6 +508,8 @@ def fill_step(step: Step, meta: MetaBuffers, entries: Sequence[StepEntry], table
     allocated again from its former self (without it rows are always rewritten whole).
     ``lookahead``: the tables also carry the pages of this many positions past the step's, for
     further decode steps that the device advances to by itself.
+    ``shared`` (single tokens without padding): the entries as groups of neighbours ``(how many, keys)`` whose first so many keys
+    lie in the same pages.
     Returns how many logits rows each entry gets."""
     B = len(entries)
     q_lens = [len(e.token_ids) for e in entries]
@@ -534,6 +562,24 @@ def fill_step(step: Step, meta: MetaBuffers, entries: Sequence[StepEntry], table
         tok[p:] = 0
         pos[p:] = 0
         host[off["seq_of_token"]:off["seq_of_token"] + N] = np.repeat(count[:Bp], lens)
+
+    groups = None
+    if shared is not None:
+        if not singles or Bp != B or sum(n for n, _ in shared) != B or min(n for n, _ in shared) < 1:
+            raise ValueError("groups of shared pages are made of all entries of a step of single tokens, without padding")
+        first, own = 0, 1
+        for n, keys in shared:
+            if not 0 <= keys <= min(starts_of[first:first + n]) + 1:
+                raise ValueError(f"{keys} shared keys are more than a sequence of their group holds")
+            own = max(own, max(starts_of[first:first + n]) + 1 - keys)
+            first += n
+        G = len(shared)
+        host[off["cu_groups"]] = 0
+        host[off["cu_groups"] + 1:off["cu_groups"] + G + 1] = np.cumsum([n for n, _ in shared])
+        host[off["shared_lens"]:off["shared_lens"] + G] = [keys for _, keys in shared]
+        cells = lambda keys, cell: -(-keys // cell) * cell
+        groups = SharedShape(G, max(n for n, _ in shared), cells(max(keys for _, keys in shared), SharedShape.SHARED_CELL),
+                             cells(own, SharedShape.OWN_CELL))
 
     counts, rows = [], []
     for b, e in enumerate(entries):
@@ -590,7 +636,10 @@ def fill_step(step: Step, meta: MetaBuffers, entries: Sequence[StepEntry], table
     step.host_token_ids = tok.copy()
     step.prefill_seqs = prefill
     live = [ctx_of[b] for b in decode if ctx_of[b] > 0]
-    step.decode_shape = DecodeShape(len(live), max(live, default=0), sum(live))
+    step.decode_shape = DecodeShape(len(live), max(live, default=0), sum(live), groups)
+    step.shared = None
+    if groups is not None:
+        step.shared = SharedPages(meta.view("cu_groups", groups.groups + 1), meta.view("shared_lens", groups.groups), groups)
     step.max_position = max(ctx_of)
     step.scratch = {}
     step._meta, step._turn, step._extra_used = meta, turn, 0

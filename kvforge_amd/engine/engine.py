@@ -16,12 +16,13 @@ from typing import Any, Sequence
 
 from kvforge_amd.config.engine import EngineConfig
 from kvforge_amd.engine.batch import StepEntry
+from kvforge_amd.engine.beams import BeamOutput, BeamSearcher
 from kvforge_amd.engine.metrics import CostModel, MetricsCollector
 from kvforge_amd.engine.request import Request, RequestOutput
 from kvforge_amd.engine.runner import ModelRunner
 from kvforge_amd.engine.scheduler import Plan, Scheduler
 from kvforge_amd.models.transformer import Transformer
-from kvforge_amd.sampling.params import SamplingParams
+from kvforge_amd.sampling.params import BeamParams, SamplingParams
 from kvforge_amd.sampling.sampler import Sampler
 from kvforge_amd.weights.random_init import write_random_model
 
@@ -49,6 +50,7 @@ class InferenceEngine:
                                    device_runs=self.runner.takes_runs)
         self.metrics = MetricsCollector()
         self._num_added = 0
+        self._beams: BeamSearcher | None = None
         self.stalled = False      # the last step found requests but nothing to plan
 
     # ------------------------------------------------------------------ construction
@@ -141,6 +143,18 @@ class InferenceEngine:
                     f"nothing can be planned although {self.scheduler.num_waiting} request(s) "
                     f"wait and {self.scheduler.num_running} run: the scheduler is stuck")
         return [final[rid] for rid in order if rid in final]
+
+    def beam_search(self, prompts: Sequence[Prompt], params: BeamParams | None = None) -> list[BeamOutput]:
+        """Search the prompts' continuations (see ``BeamParams``) to their ends; one output per prompt, its sequences best first.
+        Requests that were added meanwhile keep their pages and wait; raises ``ValueError`` where a search does not fit
+        into what is free."""
+        params = params if params is not None else BeamParams()
+        if self._beams is None:
+            self._beams = BeamSearcher(self.runner)
+        eos = getattr(self.tokenizer, "eos_token_id", None) if self.tokenizer is not None else self.model.config.eos_token_id
+        stops = set() if params.ignore_eos else {*params.stop_token_ids, *([] if eos is None else [eos])}
+        found = self._beams.run([self._token_ids(p) for p in prompts], params, stops)
+        return [s.output(self.tokenizer) for s in found]
 
     # ------------------------------------------------------------------ one step
     def step(self) -> list[RequestOutput]:

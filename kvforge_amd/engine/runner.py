@@ -106,7 +106,7 @@ class ModelRunner:
         return self.cache.slots.slot(request_id) if self.cache.slots.num_slots else -1
 
     def build_step(self, entries: Sequence[StepEntry], pad_to: int | None = None,
-                   lookahead: int = 0) -> tuple[Step, list[int]]:
+                   lookahead: int = 0, shared: "Sequence[tuple[int, int]] | None" = None) -> tuple[Step, list[int]]:
         for e in entries:
             if e.start_pos + len(e.token_ids) + lookahead > self.max_model_len:
                 raise ValueError(f"request {e.request_id} would pass max_model_len "
@@ -114,18 +114,20 @@ class ModelRunner:
         step = Step()
         step.ws, step.act_dtype, step.device = self.ws, self.model.dtype, self.device
         counts = fill_step(step, self.meta, entries, self.cache.block_table, self._slot_of,
-                           self.block_size, pad_to, self._windowed, self.cache.serial, lookahead)
+                           self.block_size, pad_to, self._windowed, self.cache.serial, lookahead, shared)
         return step, counts
 
     @torch.inference_mode()
-    def step(self, entries: Sequence[StepEntry]) -> torch.Tensor:
+    def step(self, entries: Sequence[StepEntry], shared: "Sequence[tuple[int, int]] | None" = None) -> torch.Tensor:
         """One forward over the entries; fp32 logits ``[sum of wanted places, vocab]``, rows in
-        entry order then place order.  The tensor is a view of memory the next step reuses."""
+        entry order then place order.  The tensor is a view of memory the next step reuses.
+        ``shared``: for single tokens, the entries as groups of neighbours ``(how many, keys)`` whose first so many keys lie in
+        the same pages (beams of a request): attention reads these once a group."""
         self._queued = None  # whatever is queued ahead is not what comes next
         if self._captures_step(entries):
-            logits = self._singles_step(entries)
+            logits = self._singles_step(entries, shared)
         else:
-            step, _ = self.build_step(entries)
+            step, _ = self.build_step(entries, shared=shared)
             logits = self.model.forward(step)
         self.num_forward_passes += 1
         self.num_tokens_processed += sum(len(e.token_ids) for e in entries)
@@ -138,7 +140,7 @@ class ModelRunner:
                 and all(len(e.token_ids) == 1 and e.want == "last" for e in entries)
                 and not torch.cuda.is_current_stream_capturing())
 
-    def _singles_step(self, entries: Sequence[StepEntry]) -> torch.Tensor:
+    def _singles_step(self, entries: Sequence[StepEntry], shared: "Sequence[tuple[int, int]] | None" = None) -> torch.Tensor:
         """A step of single tokens without sampling, for a caller that picks tokens by itself.  Such steps come
         again and again with the same launches, which the host makes more slowly than the device runs them (12 to 15
         us each; batch 1 of a small model 0.36 ms a step and 0.16 from a graph, batch 8 at the 1B shape 1.03 and 0.81,
@@ -147,7 +149,7 @@ class ModelRunner:
         replayed from then on.  A capture costs 0.2 to 0.9 ms beyond the step, which four replays make up for: kinds that come
         less often never pay it, and one whose graph gave way to another's before it had paid is captured later the
         next time.  The graphs of the ``STEP_GRAPHS`` kinds used last are kept, none beyond the workspace it was made with."""
-        step, _ = self.build_step(entries, pad_to=len(entries))
+        step, _ = self.build_step(entries, pad_to=len(entries), shared=shared)
         key = (len(entries), self.model.launch_key(step.decode_shape))
         if self._step_moves != self.ws.moves:
             if self.step_graphs:

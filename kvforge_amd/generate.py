@@ -37,6 +37,9 @@ def parse_args(argv: list[str] | None = None) -> argparse.Namespace:
     p.add_argument("--temperature", type=float, default=0.0)
     p.add_argument("--top-k", type=int, default=0)
     p.add_argument("--top-p", type=float, default=1.0)
+    p.add_argument("--beams", type=int, default=None, help="search with so many beams instead of sampling")
+    p.add_argument("--length-penalty", type=float, default=1.0, help="of a beam search: scores are sums over length to this power")
+    p.add_argument("--early-stopping", action="store_true", help="end a beam search once as many beams have ended as it follows")
     p.add_argument("--ignore-eos", action="store_true")
     p.add_argument("--stop-token-ids", default="", help="comma-separated token ids")
     p.add_argument("--seed", type=int, default=0)
@@ -59,6 +62,30 @@ def parse_args(argv: list[str] | None = None) -> argparse.Namespace:
 
 def _ids(text: str) -> list[int]:
     return [int(t) for t in text.replace(",", " ").split()]
+
+
+def _search(args, engine, name: str, prompts: list) -> int:
+    """``--beams``: the prompts' best continuations."""
+    from kvforge_amd.sampling.params import BeamParams
+
+    params = BeamParams(width=args.beams, max_tokens=args.max_tokens, length_penalty=args.length_penalty,
+                        early_stopping=args.early_stopping, ignore_eos=args.ignore_eos,
+                        stop_token_ids=_ids(args.stop_token_ids))
+    outs = engine.beam_search(prompts, params)
+    if args.json:
+        print(json.dumps({"model": name, "outputs": [
+            {"prompt_token_ids": o.prompt_token_ids, "sequences": [
+                {"output_token_ids": s.output_token_ids, "log_prob": s.log_prob, "score": s.score,
+                 "finish_reason": s.finish_reason.value, "text": s.text} for s in o.sequences]} for o in outs]}))
+        return 0
+    print(f"kvforge_amd: model={name} beams={args.beams} dtype={args.dtype}")
+    for n, o in enumerate(outs):
+        print(f"prompt {n}: {len(o.prompt_token_ids)} tokens")
+        for s in o.sequences:
+            print(f"  {s.score:9.4f} [{s.finish_reason.value}] {s.output_token_ids}")
+            if s.text is not None:
+                print(f"            text: {s.text!r}")
+    return 0
 
 
 def main(argv: list[str] | None = None) -> int:
@@ -91,6 +118,8 @@ def main(argv: list[str] | None = None) -> int:
         preset = args.preset or "tiny-a"
         engine = InferenceEngine.from_config(preset, config, tokenizer)
         name = f"{preset}-random(seed={args.seed})"
+    if args.beams is not None:
+        return _search(args, engine, name, prompts)
     params = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature,
                             top_k=args.top_k, top_p=args.top_p, ignore_eos=args.ignore_eos,
                             stop_token_ids=_ids(args.stop_token_ids))

@@ -28,6 +28,11 @@ from kvforge_amd.registry import register_mixer
 KEYS_PER_CUT = 512
 MAX_CUTS = 64            # what the merge kernels take
 SKEW_MAX_CUTS = 8
+# Sequences that share their first pages go to the kernel that reads these once a group from so many shared keys on (against
+# the kernel that reads every sequence's by themselves: bf16, heads of 64, one request of 4 beams, 512 shared keys 7.3 and 7.0
+# us, 1,024 7.3 and 9.8; 16 of 8 beams, 256 shared keys 10.2 and 11.5, 4,096 29 and 79).  In 32 bits always (4 beams, 16 keys 8.1
+# and 10.5, 4,096 11.2 and 31.2).
+SHARED_FROM = 512
 
 
 def compute_units(device) -> int:
@@ -389,6 +394,8 @@ class PagedAttention(Mixer):
             mods.add("convkv")
         if dtype == torch.bfloat16:
             mods |= {"gemm_bf16", "gemm_tile", "attn_mfma"}
+        if not (self.window or self.chunk):
+            mods.add("attn_beams")
         return mods
 
     def num_bytes(self) -> int:
@@ -411,11 +418,20 @@ class PagedAttention(Mixer):
             self.w_head_gate = ops.streamed(ops.plain_of(self.w_head_gate))
 
     # ------------------------------------------------------------------ launch planning
-    def launch_key(self, shape) -> tuple[int, int]:
+    def _reads_shared(self, shared) -> bool:
+        """Whether the keys that sequences share (``SharedShape``) are read once a group: plain scores over all keys (and
+        this class's own order of work)."""
+        return (shared is not None and type(self).forward is PagedAttention.forward and not (self.window or self.chunk) and self.slopes is None and not self.score_cap
+                and self.dist is None and self.score_slopes is None and self.distance_bias is None and self.d <= 256
+                and shared.max_shared > (0 if ops.plain_of(self.w_qkv).dtype == torch.float32 else SHARED_FROM))
+
+    def launch_key(self, shape):
         """(context cell, cuts for uneven contexts): all that this part's decode launches depend
         on besides the padded batch size.  A cell is ``KEYS_PER_CUT`` keys of the longest
         context (of the window, for a windowed layer), and the plan is made for the cell's lower
-        edge."""
+        edge.  Where sequences share pages, and the kernel for it is taken, what there is of them."""
+        if self._reads_shared(shape.groups):
+            return shape.groups
         seen = self.window or self.chunk
         ctx = min(shape.max_ctx, seen + self.keep_first) if seen else shape.max_ctx
         cell = min(ctx // KEYS_PER_CUT, MAX_CUTS)
@@ -503,6 +519,18 @@ class PagedAttention(Mixer):
             gates = ws.buf("attn_head_gates", (n, self.w_head_gate.shape[0]), torch.float32)
             out.append(((self.prefix, "head_gates"), x, self.w_head_gate, gates, "store"))
         return out
+
+    def _attend_shared(self, qkv, step, layer: LayerState, table, out, shared) -> None:
+        """Attention of single tokens whose sequences share pages."""
+        H, KV, d, n, s = self.H, self.KV, self.d, step.n_seqs, shared.shape
+        key = ("attention.shared_cuts", H, KV, d, qkv.dtype)
+        cuts = step.scratch.get(key)
+        if cuts is None:
+            cuts = step.scratch[key] = ops.attn_beams_cuts(qkv, layer.k_pages, H, KV, d, s.groups, n, s.widest, s.max_shared, s.max_own)
+        parts = n * H * sum(cuts)
+        workspace = (step.ws.buf("shared_part_acc", (parts * d,), torch.float32), step.ws.buf("shared_part_ml", (parts * 2,), torch.float32))
+        ops.attn_beams(qkv, layer.k_pages, layer.v_pages, table, shared.cu_groups, shared.shared_lens, step.ctx_lens, out, H, KV, d,
+                       self.scale, s.widest, cuts, workspace, sinks=self.sinks)
 
     def forward(self, x, step, layer: LayerState, residual) -> None:
         """``x``: normalised activations, or (after ``absorb_norm``) the fp32 residual stream."""
@@ -597,7 +625,11 @@ class PagedAttention(Mixer):
                              work, out, H, KV, d, self.scale, window, self.slopes, rows_per_item,
                              keep_first=self.keep_first, gate=gate_in_kernel, sinks=self.sinks,
                              score_cap=self.score_cap, chunk=chunk, dist=self.dist)
-        if step.n_decode:
+        shared = step.shared if step.shared is not None and self._reads_shared(step.shared.shape) else None
+        if shared is not None:
+            gate_in_kernel = None
+            self._attend_shared(qkv, step, layer, table, out, shared)
+        elif step.n_decode:
             splits, in_order = self._decode_plan(step, ops.attention_on_matrix_cores(act, bs, d))
             token_is_seq = step.decode_seq_ids is None and work is None
             order = step.decode_order if in_order and token_is_seq else None

@@ -73,3 +73,48 @@ def attend(q, k_pages, v_pages, tables, ctx_lens, heads, kv_heads, dim, scale, s
             out[i, h * dim:(h + 1) * dim] = p @ v
             weight[i, h * dim:(h + 1) * dim] = p @ v.abs()
     return out, weight
+
+
+def search(next_logits, prompt, width, max_tokens, length_penalty=1.0, early_stopping=False, stops=()):
+    """Beam search by its definition: ``next_logits(tokens)`` are the logits behind a whole sequence.  Returns the ended
+    sequences ``(output tokens, log-probability, score, reason)``, best first, and the smallest difference that a choice went
+    by: of the last candidate that was taken and the first that was not, of scores that were ranked, of the best living
+    score and the worst ended one (what a search with other rounding may choose otherwise)."""
+    beams, ended, gap = [((), 0.0)], [], math.inf
+    for step in range(1, max_tokens + 1):
+        everyone = []
+        for b, (tokens, log_prob) in enumerate(beams):
+            lp = torch.log_softmax(next_logits(list(prompt) + list(tokens)).double(), dim=0)
+            best = torch.sort(lp, descending=True, stable=True).indices[:2 * width + 1].tolist()
+            everyone += [(log_prob + float(lp[t]), b, t) for t in best]
+        everyone.sort(key=lambda c: (-c[0], c[1], c[2]))
+        following, left = [], None
+        for rank, (log_prob, b, token) in enumerate(everyone[:2 * width]):
+            tokens = beams[b][0] + (token,)
+            if token in stops:
+                if rank < width:
+                    ended.append((list(tokens), log_prob, log_prob / step ** length_penalty, "stop"))
+            elif len(following) < width:
+                following.append((tokens, log_prob))
+            elif left is None:
+                left = log_prob
+        if left is not None:
+            gap = min(gap, following[-1][1] - left)
+        for at in (width, 2 * width):         # what may end is cut off there, and what is looked at
+            if len(everyone) > at and (at == width and (everyone[at - 1][2] in stops or everyone[at][2] in stops) or at > width and left is None):
+                gap = min(gap, everyone[at - 1][0] - everyone[at][0])
+        if step == max_tokens:
+            ended += [(list(t), p, p / step ** length_penalty, "length") for t, p in following]
+        ended = sorted(ended, key=lambda e: -e[2])
+        gap = min([gap] + [a[2] - b[2] for a, b in zip(ended, ended[1:width + 1])])
+        ended = ended[:width]
+        if step == max_tokens or not following:
+            break
+        if len(ended) == width:
+            best = max(p for _, p in following) / step ** length_penalty
+            if not early_stopping:
+                gap = min(gap, abs(best - ended[-1][2]))
+            if early_stopping or best <= ended[-1][2]:
+                break
+        beams = following
+    return ended, gap

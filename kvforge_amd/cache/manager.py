@@ -18,6 +18,21 @@ from kvforge_amd.cache.block_pool import BlockPool, NoFreeBlocksError
 RELEASED = -1  # table entry of a page that was given back (or never held)
 
 
+def common_start(a: list, b: list) -> int:
+    """How many entries at the start of two lists are the same."""
+    n = min(len(a), len(b))
+    if a[:n] == b[:n]:
+        return n
+    lo, hi = 0, n - 1            # lo are the same, not all of hi + 1
+    while lo < hi:
+        mid = (lo + hi + 1) // 2
+        if a[lo:mid] == b[lo:mid]:
+            lo = mid
+        else:
+            hi = mid - 1
+    return lo
+
+
 @dataclass(frozen=True)
 class CacheGroup:
     """Layers whose mixers have equal cache needs.  ``layers``: places in the model's run order
@@ -213,21 +228,22 @@ class CacheManager:
         if self._num_tokens[parent_id] < num_tokens:
             raise ValueError(f"request {parent_id} holds {self._num_tokens[parent_id]} tokens, not {num_tokens}")
         whole, need = num_tokens // self.block_size, self.blocks_needed(num_tokens)
-        known = request_id in self._num_tokens
         for g, p in enumerate(self.pools):
             if len(self._tables[g][parent_id]) != need:
                 raise ValueError(f"the tables of {parent_id} hold more or fewer pages than {num_tokens} tokens need")
-            own = sum(b != RELEASED and p.ref_count(b) == 1 for b in self._tables[g][request_id]) if known else 0
-            if need - whole > p.num_free + own:
-                raise NoFreeBlocksError(f"no page for {request_id} to go on from {parent_id}")
+            if need - whole > p.num_free:
+                own = sum(b != RELEASED and p.ref_count(b) == 1 for b in self._tables[g].get(request_id, ()))
+                if need - whole > p.num_free + own:
+                    raise NoFreeBlocksError(f"no page for {request_id} to go on from {parent_id}")
         if self.slots.num_slots and not self.slots.has(request_id):
             self.slots.take(request_id)
         for g, p in enumerate(self.pools):
-            table = self._tables[g][parent_id][:whole]
-            for b in table:
+            table, before = self._tables[g][parent_id][:whole], self._tables[g].get(request_id, [])
+            same = common_start(table, before)         # (the pages of a search's prompt stay as they are)
+            for b in table[same:]:
                 if b != RELEASED:
                     p.share(b)
-            for b in reversed(self._tables[g].get(request_id, ())):
+            for b in reversed(before[same:]):
                 if b != RELEASED:
                     p.release(b)
             if need > whole:
@@ -245,11 +261,8 @@ class CacheManager:
         for g, group in enumerate(self.groups):
             if group.window is not None:
                 continue
-            tables = [self._tables[g][r] for r in request_ids]
-            most = min(map(len, tables))
-            i = min(known, most)
-            while i < most and all(t[i] == tables[0][i] for t in tables):
-                i += 1
+            first, *others = [self._tables[g][r][known:] for r in request_ids]
+            i = known + min((common_start(first, t) for t in others), default=len(first))
             n = i if n is None else min(n, i)
         return n or 0
 

@@ -153,7 +153,7 @@ class BeamSearcher:
         for s, i, by in moves:
             for to, p in by.items():
                 cache.branch(i[to], i[p], len(s.prompt) + s.length - 1)
-        kinds = [g for g in range(cache.num_groups)] + ([-1] if self.states is not None else [])
+        kinds = [*range(cache.num_groups), *([-1] if self.states is not None else [])]       # (-1: state slots)
         if not any(by for _, _, by in moves) or not kinds:
             return
         table = np.full((len(kinds), 2, len(searches), width), -1, dtype=np.int32)

@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from kvforge_amd.cache import RELEASED, CacheGroup, CacheManager, NoFreeBlocksError
+from kvforge_amd.cache.manager import common_start
 from kvforge_amd.engine.batch import DecodeShape, MetaBuffers, SharedShape, Step, StepEntry, fill_step
 from kvforge_amd.engine.beams import BeamSearcher, Search
 from kvforge_amd.kernels import ops
@@ -257,6 +258,15 @@ def test_no_page_is_lost_in_random_searches(seed):
     for rid in live:
         m.free(rid)
     assert all(p.num_free == p.num_blocks for p in m.pools) and m.slots.num_free == 16
+
+
+def test_the_common_start_of_two_lists():
+    rng = random.Random(1)
+    for _ in range(400):
+        a = [rng.randrange(3) for _ in range(rng.randrange(9))]
+        b = a[:rng.randrange(len(a) + 1)] + [rng.randrange(3) for _ in range(rng.randrange(4))]
+        want = next((i for i, (x, y) in enumerate(zip(a, b)) if x != y), min(len(a), len(b)))
+        assert common_start(a, b) == common_start(b, a) == want
 
 
 # ------------------------------------------------------------------------------------- the choice of beams

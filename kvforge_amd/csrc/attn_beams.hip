@@ -102,20 +102,14 @@ template <typename T> struct Tensors {
   float2* ml;
 };
 
-// The sequence of [first, first + n) whose pages the group's `shared` keys are read from: the first that holds as many, or else the
-// one that holds the most.
+// The first of the sequences [first, first + n) that holds `shared` keys, from whose pages the group's are read; -1: none.
 __device__ __forceinline__ int holder_of(int first, int n, int shared, const int* __restrict__ ctx_lens) {
   const int lane = threadIdx.x % KVF_WAVE;
   for (int i = 0; i < n; i += KVF_WAVE) {
     const unsigned long long held = __ballot(i + lane < n && ctx_lens[first + min(i + lane, n - 1)] >= shared);
     if (held) return first + i + __ffsll(static_cast<long long>(held)) - 1;
   }
-  int most = 0, who = first;
-  for (int i = first; i < first + n; ++i) {
-    const int c = ctx_lens[i];
-    if (c > most) most = c, who = i;
-  }
-  return who;
+  return -1;
 }
 
 // What a wave holds of 16 * RT rows: Q, and the running reference, sum and accumulator of each.
@@ -127,7 +121,7 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
   typename F::Part q[RT][SLICES];
   f32x4 acc[RT][DT];
   float m[RT], sum[RT];
-  int ctx[RT];           // keys of the row's sequence
+  bool live[RT];         // whether the row's sequence holds enough keys to take part
 
   // A lane's part of a row from element e on, zeros behind the head's end (read inside it all the same).
   static __device__ __forceinline__ bool has(int j, int tiles) { return FORM == WHOLE || j < tiles; }
@@ -137,14 +131,14 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
     return e < d ? v : F::zero();
   }
 
-  // Rows [row0, row0 + 16 RT) of `rows`: sequence first + row / G, head row % G of kv head `kvh`.
-  __device__ __forceinline__ void start(const Tensors<T>& t, const Args& a, int first, int rows, int row0, int kvh) {
+  // Rows [row0, row0 + 16 RT) of `rows`, those of sequences of `least` keys and more: sequence first + row / G, head row % G of kv head `kvh`.
+  __device__ __forceinline__ void start(const Tensors<T>& t, const Args& a, int first, int rows, int row0, int kvh, int least) {
     const int lane = threadIdx.x % KVF_WAVE, g = lane / 16, r = lane % 16, G = a.G;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int row = min(row0 + rt * 16 + r, rows - 1);
       const int seq = group_of(row, a);
-      ctx[rt] = t.ctx_lens[first + seq];
+      live[rt] = t.ctx_lens[first + seq] >= least;
       const T* from = t.q + static_cast<long>(first + seq) * a.q_stride + (kvh * G + row - seq * G) * a.d;
 #pragma unroll
       for (int c = 0; c < SLICES; ++c) q[rt][c] = part(from, c * F::SLICE + g * LANE_D, a.d);
@@ -233,10 +227,6 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
 #pragma unroll
           for (int c = 0; c < SLICES; ++c) s[rt][tt] = F::scores(kf[tt][c], q[rt][c], s[rt][tt]);
         }
-      // (rows of sequences that are shorter than what their group shares see no more than their own keys)
-      bool all_rows = whole;
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) all_rows &= static_cast<bool>(__all(kb + BLOCK <= ctx[rt]));
       if (next < hi) load_k(next, pk_next);
       typename F::Probs pf[RT];
 #pragma unroll
@@ -244,9 +234,9 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
           s[rt][tt] *= a.scale2;
-          if (!all_rows)
+          if (!whole)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[rt][tt][i] = (keep >> (4 * tt + i) & 1u) && kb + 8 * g + 4 * tt + i < ctx[rt] ? s[rt][tt][i] : -INFINITY;
+            for (int i = 0; i < 4; ++i) s[rt][tt][i] = keep >> (4 * tt + i) & 1u ? s[rt][tt][i] : -INFINITY;
         }
         float most = s[rt][0][0];
 #pragma unroll
@@ -292,7 +282,7 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
   }
   // (reference, sum over all keys of the cut), -inf where there are none (NaN stays NaN); whether there is an accumulator.
   __device__ __forceinline__ bool leave_sum(const Tensors<T>& t, int rt, long at, float top, float total, bool writes) const {
-    const bool any = ctx[rt] > 0 && (total > 0.f || total != total);
+    const bool any = live[rt] && (total > 0.f || total != total);
     if (writes && at >= 0) t.ml[at] = any ? make_float2(top > -INFINITY ? top : 0.f, total) : make_float2(-INFINITY, 0.f);
     return any && at >= 0;
   }
@@ -328,13 +318,14 @@ __global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 
     if (n == 0) return;
     const int rows = n * G, tiles = a.d / 16;
     int lo = 0, hi = min(max(t.shared_lens[group], 0), most);
-    const int holder = holder_of(first, n, hi, t.ctx_lens);
+    const int shared = max(hi, 1), holder = holder_of(first, n, shared, t.ctx_lens);
+    if (holder < 0) hi = 0;
     cut_of(lo, hi, cut, a.cs, WAVES * BLOCK);
     for (int row0 = block * 16 * RT; row0 < rows; row0 += a.blocks * 16 * RT) {
       typedef Rows<T, DT, RT, FORM> Held;
       Held x;
-      x.start(t, a, first, rows, row0, kvh);
-      x.walk(t, a, t.table + static_cast<long>(holder) * a.width, kvh, lo + wave * BLOCK, WAVES * BLOCK, lo, hi);
+      x.start(t, a, first, rows, row0, kvh, shared);
+      x.walk(t, a, t.table + static_cast<long>(max(holder, 0)) * a.width, kvh, lo + wave * BLOCK, WAVES * BLOCK, lo, hi);
       // the waves' results: tile j of the elements is summed by wave j % WAVES
       float l[RT];
 #pragma unroll
@@ -396,12 +387,12 @@ __global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 
       for (int i = lane; i < G * a.cs; i += KVF_WAVE)
         t.ml[(static_cast<long>(seq) * a.H + kvh * G + i / a.cs) * (a.cs + a.co) + i % a.cs] = make_float2(-INFINITY, 0.f);
     int hi = max(min(t.ctx_lens[seq], most), 0);
-    lo = min(lo, hi);
+    if (lo > hi) lo = 0;          // shorter than what its group shares: all of its keys are its own
     cut_of(lo, hi, cut, a.co, BLOCK);
     for (int row0 = 0; row0 < G; row0 += 16) {
       typedef Rows<T, DT, 1, FORM> Held;
       Held x;
-      x.start(t, a, seq, G, row0, kvh);
+      x.start(t, a, seq, G, row0, kvh, 1);
       x.walk(t, a, t.table + static_cast<long>(seq) * a.width, kvh, lo & ~7, BLOCK, lo, hi);
       const long at = x.place(a, 0, seq, G, row0, kvh, a.cs + cut);
       const float total = x.whole_sum(0);       // (all lanes take part)
@@ -559,7 +550,7 @@ KVF_EXPORT int kvf_attn_beams(int bf16, const void* q, const void* k, const void
   if (KV < 1 || H < KV || H % KV || d < 16 || d > 256 || d % 16 || bs < 1 || nb < 1 || width < 0 || n_seqs < 0 || n_groups < 0 ||
       widest < 1 || cs < 0 || co < 1 || cs > 64 || co > 64 || (n_groups == 0 && cs))
     return static_cast<int>(hipErrorInvalidValue);
-  if (static_cast<long>(width) * bs >= (1L << 31) - 1024 || static_cast<long>(width) * bs * bs >= (1L << 32)) return static_cast<int>(hipErrorInvalidValue);
+  if (static_cast<long>(width) * bs >= 1L << 30 || static_cast<long>(width) * bs * bs >= (1L << 32)) return static_cast<int>(hipErrorInvalidValue);
   if (n_seqs == 0) return 0;
   const long rows = static_cast<long>(widest) * (H / KV);
   if (rows > 1 << 20) return static_cast<int>(hipErrorInvalidValue);

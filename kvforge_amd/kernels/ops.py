@@ -1796,7 +1796,7 @@ def attn_beams(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     """Attention of one token per sequence (row ``i`` of ``q`` is sequence ``i``'s) over ``ctx_lens[i]`` cached keys, for
     sequences in groups ``cu_groups[g] .. cu_groups[g + 1] - 1`` whose first ``shared_lens[g]`` keys are the same, as the beams
     of a request have them behind its prompt: these are read once for the whole group, from the pages of its first
-    sequence that holds any.  (One that is shorter than what its group shares attends over as many of the shared keys as it holds.)  A sequence without keys gets zeros; one that no group names shares nothing.  Page numbers outside the
+    sequence that holds as many.  (One that is shorter than what its group shares is read by itself.)  A sequence without keys gets zeros; one that no group names shares nothing.  Page numbers outside the
     pages stand for keys that are not there.  ``widest``: sequences of the largest group (it decides how workgroups are laid out,
     results do not depend on it).  ``cuts`` from ``attn_beams_cuts``, ``workspace`` from ``attn_beams_workspace``; launches that
     share a workspace must not overlap.  ``sinks``: as in ``attn_prefill``.  Pages of any number of tokens (multiples of 8 are
@@ -1818,7 +1818,7 @@ def attn_beams(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
         raise KernelError("attn_beams: at least one page; pages start on 16 bytes")
     _check(block_table, "block_table", I32, (n, None))
     width = block_table.shape[1]
-    if width * bs >= 2**31 - 1024 or width * bs * bs >= 2**32:
+    if width * bs >= 2**30 or width * bs * bs >= 2**32:
         raise KernelError(f"attn_beams: {width} pages of {bs} tokens a sequence are more than the kernel counts")
     _check(cu_groups, "cu_groups", I32, (None,))
     groups = cu_groups.shape[0] - 1

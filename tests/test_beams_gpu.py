@@ -82,6 +82,14 @@ def test_selection_of_beams_of_their_own_number_dead_ones_and_none():
     assert outs[1][[1, 2, 4, 5]].eq(-1).all()
 
 
+@pytest.mark.parametrize("rows,cu,vocab,count", [(150, [0, 70, 71, 150], 900, 20), (300, [0, 300], 70, 64), (64, [0, 64], 9000, 32)])
+def test_selection_of_more_beams_than_are_merged_at_a_time(rows, cu, vocab, count):
+    g = torch.Generator().manual_seed(rows)
+    logits = (torch.randn(rows, vocab, generator=g) * 2).to(DEV)
+    scores = (-torch.rand(rows, generator=g) * 3).to(DEV)
+    check_select(logits, scores, cu, count, run_select(logits, scores, cu, count))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("vocab", [70, 2500, 20000])
 def test_selection_of_rows_with_ruled_out_and_infinite_logits(dtype, vocab):
@@ -302,8 +310,8 @@ def test_attention_over_pages_of_any_size_in_any_cuts(dtype, page, cuts):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_shared_lengths_inside_a_page_and_beyond_a_sequence(dtype):
-    """Any number of first keys may be shared, the table rows of a group agreeing on them; a sequence that is shorter bounds
-    what is."""
+    """Any number of first keys may be shared, the table rows of a group agreeing on them; a sequence that is shorter is read
+    by itself, and what others hold behind its end does not reach it."""
     H, KV, d = 4, 2, 32
     k, v, tables, cu, shared, ctx = paged([(64, [70, 90, 66]), (32, [40, 33])], KV, d, 16, dtype, 9)
     q = torch.randn(len(ctx), H * d, generator=torch.Generator().manual_seed(4)).to(dtype)
@@ -319,6 +327,25 @@ def test_shared_lengths_inside_a_page_and_beyond_a_sequence(dtype):
     for few in ([20, 70, 66] + ctx[3:], [17, 30, 50] + ctx[3:], [0, 0, 40] + ctx[3:]):
         out = run_attend(q, k, v, short, cu, [64, 32], few, H, KV, d, 0.3)
         check_attend(out, q, k, v, short, few, H, KV, d, 0.3)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_infinities_behind_a_short_sequence_stay_with_the_long_ones(dtype):
+    H, KV, d = 4, 2, 32
+    k, v, tables, cu, shared, ctx = paged([(64, [70, 90, 66])], KV, d, 16, dtype, 9)
+    q = torch.randn(3, H * d, generator=torch.Generator().manual_seed(4)).to(dtype)
+    v[tables[0][3], :, :, 5], k[tables[0][2], :, 3] = math.inf, math.nan
+    few, same = [70, 20, 40], [tables[0]] * 3
+    out = run_attend(q, k, v, same, cu, [64], few, H, KV, d, 0.3).cpu()
+    assert out[0].isnan().all()
+    k[tables[0][2], :, 3] = 0.0
+    want, weight = plain.attend(q, k, v, same, few, H, KV, d, 0.3)
+    for i in (1, 2):
+        bound = 2.5e-5 * weight[i] + 1e-7 + (2.0 ** -8 * (weight[i] + 1.01 * want[i].abs()) if dtype == BF16 else 0.0)
+        assert i == 2 or bool(((out[i].double() - want[i]).abs() <= bound).all())
+    out = run_attend(q, k, v, same, cu, [64], few, H, KV, d, 0.3).cpu()
+    assert not out[0].isfinite().any() and bool(((out[1:].double() - want[1:]).abs() <= 2.5e-5 * weight[1:] + 1e-7 + (
+        2.0 ** -8 * (weight[1:] + 1.01 * want[1:].abs()) if dtype == BF16 else 0.0)).all())
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -372,6 +372,10 @@ __global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 
     const int item = (blockIdx.x - shared_items) * WAVES + wave;
     const int kvh = item % a.KV, cut = item / a.KV % a.co, seq = item / a.KV / a.co;
     if (seq >= a.n_seqs) return;
+    typedef Rows<T, DT, 1, FORM> Held;
+    Held x;
+    x.start(t, a, seq, G, 0, kvh, 1);        // (loaded while the group is looked for)
+    const int ctx = t.ctx_lens[seq];
     // the group that the sequence is in
     int lo = 0;
     bool grouped = false;
@@ -386,13 +390,11 @@ __global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 
     if (!grouped && cut == 0)       // nobody else tells of its shared keys
       for (int i = lane; i < G * a.cs; i += KVF_WAVE)
         t.ml[(static_cast<long>(seq) * a.H + kvh * G + i / a.cs) * (a.cs + a.co) + i % a.cs] = make_float2(-INFINITY, 0.f);
-    int hi = max(min(t.ctx_lens[seq], most), 0);
+    int hi = max(min(ctx, most), 0);
     if (lo > hi) lo = 0;          // shorter than what its group shares: all of its keys are its own
     cut_of(lo, hi, cut, a.co, BLOCK);
     for (int row0 = 0; row0 < G; row0 += 16) {
-      typedef Rows<T, DT, 1, FORM> Held;
-      Held x;
-      x.start(t, a, seq, G, row0, kvh, 1);
+      if (row0) x.start(t, a, seq, G, row0, kvh, 1);
       x.walk(t, a, t.table + static_cast<long>(seq) * a.width, kvh, lo & ~7, BLOCK, lo, hi);
       const long at = x.place(a, 0, seq, G, row0, kvh, a.cs + cut);
       const float total = x.whole_sum(0);       // (all lanes take part)

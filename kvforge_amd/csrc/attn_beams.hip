@@ -149,8 +149,9 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
     }
   }
 
-  // Blocks kb, kb + step, ... of the keys [lo, hi) of the pages in `table`.  kb: a multiple of 8.  The page numbers of a
-  // block are looked up, and its K fragments loaded, while the block before it is worked on.
+  // Blocks kb, kb + step, ... of the keys [lo, hi) of the pages in `table`.  kb: a multiple of 8.  A block's K fragments are
+  // loaded while the block before it is worked on, its page numbers looked up one earlier still: loads come back in order, so
+  // one that waited for a number asked for in the same turn would wait for the V loads ahead of it too.
   __device__ __forceinline__ void walk(const Tensors<T>& t, const Args& a, const int* __restrict__ table, int kvh, int kb, int step, int lo, int hi) {
     const int lane = threadIdx.x % KVF_WAVE, g = lane / 16, r = lane % 16;
     const int d = FORM == WHOLE ? DT * 16 : a.d, tiles = d / 16;
@@ -182,10 +183,12 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
       }
     };
     if (kb >= hi) return;
-    int pv = 0;                          // (not for ANY) the page of keys kb + 8 g
+    int pv = 0, pk_next = 0, pv_next = 0;       // (not for ANY) the pages of keys kb + 8 g, next + 8 (r / 4), next + 8 g
     if constexpr (FORM != ANY) {
       const int pk = lookup(kb + 8 * (r / 4));
       pv = lookup(kb + 8 * g);
+      pk_next = lookup(kb + step + 8 * (r / 4));
+      pv_next = lookup(kb + step + 8 * g);
       load_k(kb, pk);
     } else {
       load_k(kb, 0);
@@ -194,17 +197,17 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
       const int next = kb + step;
       typename F::Keys vf[DT];
       unsigned keep = 0;                // which of the lane's keys kb + 8 g + (0 .. 7) count
-      int pk_next = -1, pv_next = -1;
+      int pk_after = 0, pv_after = 0;
       if constexpr (FORM != ANY) {
         const int key = kb + 8 * g, from = max(lo - key, 0), to = min(hi - key, 8);
         const bool ok = valid(pv);
         keep = ok && to > from ? (0xffu >> (8 - to)) & (0xffu << from) : 0u;
         const T* v0 = vp + (ok ? pv : 0) * page_elems + (ok ? key - page_of(key, a) * a.bs : 0) + r * a.bs;
+        pk_after = lookup(next + step + 8 * (r / 4));
+        pv_after = lookup(next + step + 8 * g);
 #pragma unroll
         for (int j = 0; j < DT; ++j)
           if (has(j, tiles)) vf[j] = F::load_keys(v0 + static_cast<long>(j) * 16 * a.bs);
-        pk_next = lookup(next + 8 * (r / 4));
-        pv_next = lookup(next + 8 * g);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -272,6 +275,8 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
       if (next >= hi) break;
       kb = next;
       pv = pv_next;
+      pk_next = pk_after;
+      pv_next = pv_after;
     }
   }
 

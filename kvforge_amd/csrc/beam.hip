@@ -772,7 +772,7 @@ KVF_EXPORT int kvf_beam_reorder(const void* tiles, int n_tiles, int rows, int re
   if (beams < 1 || beams > 32 || requests < 0 || requests > 65535 || n_tiles < 0 || rows < 0) return static_cast<int>(hipErrorInvalidValue);
   if (requests == 0 || n_tiles == 0 || beams == 1) return 0;
   const auto* t = static_cast<const Tile*>(tiles);
-  if (beams <= 4) reorder_launch<4, 4>(t, n_tiles, rows, requests, beams, slots, parents, stream);
+  if (beams <= 4) reorder_launch<4, 2>(t, n_tiles, rows, requests, beams, slots, parents, stream);
   else if (beams <= 8) reorder_launch<8, 2>(t, n_tiles, rows, requests, beams, slots, parents, stream);
   else if (beams <= 16) reorder_launch<16, 2>(t, n_tiles, rows, requests, beams, slots, parents, stream);
   else reorder_launch<32, 1>(t, n_tiles, rows, requests, beams, slots, parents, stream);

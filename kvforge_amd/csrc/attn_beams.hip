@@ -18,6 +18,8 @@
 //
 // A row's reference (what is subtracted in the exponent) is raised only when a score passes it by LAZY (in log2 units); scores,
 // sums and accumulators are fp32.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -123,13 +125,11 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
   float m[RT], sum[RT];
   bool live[RT];         // whether the row's sequence holds enough keys to take part
 
-  // A lane's part of a row from element e on, zeros behind the head's end (read inside it all the same).
+  // A lane's part of a row from element e on; behind the head's end something inside it, which `within` makes zeros (where it is
+  // used: a load that is looked at is waited for).
   static __device__ __forceinline__ bool has(int j, int tiles) { return FORM == WHOLE || j < tiles; }
-  static __device__ __forceinline__ typename F::Part part(const T* row, int e, int d) {
-    if constexpr (FORM == WHOLE) return F::load(row + e);
-    const typename F::Part v = F::load(row + min(e, d - LANE_D));
-    return e < d ? v : F::zero();
-  }
+  static __device__ __forceinline__ typename F::Part part(const T* row, int e, int d) { return F::load(row + (FORM == WHOLE ? e : min(e, d - LANE_D))); }
+  static __device__ __forceinline__ typename F::Part within(typename F::Part v, int e, int d) { return FORM == WHOLE || e < d ? v : F::zero(); }
 
   // Rows [row0, row0 + 16 RT) of `rows`, those of sequences of `least` keys and more: sequence first + row / G, head row % G of kv head `kvh`.
   __device__ __forceinline__ void start(const Tensors<T>& t, const Args& a, int first, int rows, int row0, int kvh, int least) {
@@ -141,7 +141,7 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
       live[rt] = t.ctx_lens[first + seq] >= least;
       const T* from = t.q + static_cast<long>(first + seq) * a.q_stride + (kvh * G + row - seq * G) * a.d;
 #pragma unroll
-      for (int c = 0; c < SLICES; ++c) q[rt][c] = part(from, c * F::SLICE + g * LANE_D, a.d);
+      for (int c = 0; c < SLICES; ++c) q[rt][c] = within(part(from, c * F::SLICE + g * LANE_D, a.d), c * F::SLICE + g * LANE_D, a.d);
       m[rt] = -INFINITY;
       sum[rt] = 0.f;
 #pragma unroll
@@ -159,13 +159,16 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
     const T* kp = t.k + static_cast<long>(kvh) * a.bs * d;
     const T* vp = t.v + static_cast<long>(kvh) * a.bs * d;
     typename F::Part kf[2][SLICES];
-    // the page that holds the keys from `key` on, -1 where there is none
-    auto lookup = [&](int key) { return key < hi ? table[page_of(key, a)] : -1; };
+    if (kb >= hi) return;
+    // The page that holds the keys from `key` on (that of the last key behind it).  No load depends on whether there are
+    // more keys, the last turn is one of its own: behind a branch around loads the compiler waits as if they were not asked for.
+    const int last = FORM != ANY ? page_of(hi - 1, a) : 0;
+    auto lookup = [&](int key) { return table[min(page_of(key, a), last)]; };
     auto valid = [&](int page) { return page >= 0 && page < a.nb; };
     auto load_k = [&](int at, int page) {         // page (not for ANY): that of the keys at + 8 (r / 4)
       if constexpr (FORM != ANY) {
         const int key = at + 8 * (r / 4);
-        const bool ok = valid(page);
+        const bool ok = key < hi && valid(page);
         const T* from = kp + (ok ? page : 0) * page_elems + static_cast<long>((ok ? key - page_of(key, a) * a.bs : 0) + r % 4) * d;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
@@ -182,32 +185,34 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
         }
       }
     };
-    if (kb >= hi) return;
     int pv = 0, pk_next = 0, pv_next = 0;       // (not for ANY) the pages of keys kb + 8 g, next + 8 (r / 4), next + 8 g
     if constexpr (FORM != ANY) {
       const int pk = lookup(kb + 8 * (r / 4));
       pv = lookup(kb + 8 * g);
       pk_next = lookup(kb + step + 8 * (r / 4));
       pv_next = lookup(kb + step + 8 * g);
+      asm volatile("" : "+v"(pk_next), "+v"(pv_next));       // (to have them ahead of K, not where the loop begins)
       load_k(kb, pk);
     } else {
       load_k(kb, 0);
     }
-    while (true) {
+    auto turn = [&](auto more) {        // more: there is a further block
       const int next = kb + step;
       typename F::Keys vf[DT];
       unsigned keep = 0;                // which of the lane's keys kb + 8 g + (0 .. 7) count
       int pk_after = 0, pv_after = 0;
       if constexpr (FORM != ANY) {
         const int key = kb + 8 * g, from = max(lo - key, 0), to = min(hi - key, 8);
-        const bool ok = valid(pv);
+        const bool ok = key < hi && valid(pv);
         keep = ok && to > from ? (0xffu >> (8 - to)) & (0xffu << from) : 0u;
         const T* v0 = vp + (ok ? pv : 0) * page_elems + (ok ? key - page_of(key, a) * a.bs : 0) + r * a.bs;
-        pk_after = lookup(next + step + 8 * (r / 4));
-        pv_after = lookup(next + step + 8 * g);
+        if constexpr (more) {
+          pk_after = lookup(next + step + 8 * (r / 4));
+          pv_after = lookup(next + step + 8 * g);
+        }
 #pragma unroll
         for (int j = 0; j < DT; ++j)
-          if (has(j, tiles)) vf[j] = F::load_keys(v0 + static_cast<long>(j) * 16 * a.bs);
+          vf[j] = F::load_keys(v0 + static_cast<long>(has(j, tiles) ? j : 0) * 16 * a.bs);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -217,30 +222,36 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
           const T* v0 = vp + (valid(p) ? p : 0) * page_elems + (valid(p) ? key % a.bs : 0) + r * a.bs;
 #pragma unroll
           for (int j = 0; j < DT; ++j)
-            if (has(j, tiles)) F::set(vf[j], i, v0[static_cast<long>(j) * 16 * a.bs]);
+            F::set(vf[j], i, v0[static_cast<long>(has(j, tiles) ? j : 0) * 16 * a.bs]);
         }
       }
       const bool whole = __all(keep == 0xffu);
       f32x4 s[RT][2];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+      for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
+        for (int rt = 0; rt < RT; ++rt) {
           s[rt][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int c = 0; c < SLICES; ++c) s[rt][tt] = F::scores(kf[tt][c], q[rt][c], s[rt][tt]);
+          for (int c = 0; c < SLICES; ++c) s[rt][tt] = F::scores(within(kf[tt][c], c * F::SLICE + g * LANE_D, d), q[rt][c], s[rt][tt]);
         }
-      if (next < hi) load_k(next, pk_next);
+      if constexpr (more) load_k(next, pk_next);
+      // All products are read here, ahead of any branch: hipcc 7.2 puts no wait between a product of the matrix cores and the
+      // first read of it in a block where a branch around a long one meets the long one.
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float x = s[rt][i / 4][i % 4] * a.scale2;
+          asm volatile("" : "+v"(x));
+          s[rt][i / 4][i % 4] = x;
+        }
       typename F::Probs pf[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
+        if (!whole)
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-          s[rt][tt] *= a.scale2;
-          if (!whole)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[rt][tt][i] = keep >> (4 * tt + i) & 1u ? s[rt][tt][i] : -INFINITY;
-        }
+          for (int i = 0; i < 8; ++i) s[rt][i / 4][i % 4] = keep >> i & 1u ? s[rt][i / 4][i % 4] : -INFINITY;
         float most = s[rt][0][0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) most = fmaxf(most, s[rt][i / 4][i % 4]);
@@ -265,19 +276,18 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
       }
       if (!whole)
 #pragma unroll
-        for (int j = 0; j < DT; ++j)
-          if (has(j, tiles)) F::clear(vf[j], keep);
+        for (int j = 0; j < DT; ++j) F::clear(vf[j], keep);
 #pragma unroll
-      for (int j = 0; j < DT; ++j)
-        if (has(j, tiles))
+      for (int j = 0; j < DT; ++j)        // (those behind the head's end too: nobody reads their sums)
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) acc[rt][j] = F::values(vf[j], pf[rt], acc[rt][j]);
-      if (next >= hi) break;
+        for (int rt = 0; rt < RT; ++rt) acc[rt][j] = F::values(vf[j], pf[rt], acc[rt][j]);
       kb = next;
       pv = pv_next;
       pk_next = pk_after;
       pv_next = pv_after;
-    }
+    };
+    while (kb + step < hi) turn(std::true_type{});
+    turn(std::false_type{});
   }
 
   // Where row rt * 16 + r of the rows leaves its results as cut `cut`; -1: nowhere.

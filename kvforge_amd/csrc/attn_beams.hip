@@ -17,7 +17,14 @@
 // Fragments come from the pages in this order, nothing is staged.  Lanes without a valid page read page 0 and are masked.
 //
 // A row's reference (what is subtracted in the exponent) is raised only when a score passes it by LAZY (in log2 units); scores,
-// sums and accumulators are fp32.
+// sums and accumulators are fp32.  bf16: a probability is rounded to bf16 on its way into the product with V, as the cached V is;
+// errors of different keys do not add up in one direction, and outputs are off by up to 0.0023 of their largest where rounding
+// them to bf16 alone costs 0.0017.  Two bf16 parts a probability would come down to that, for 4% of the time.
+//
+// What bounds it: the keys' bytes where there are many of them (4 x 8 beams behind 32,768 keys, 8 kv heads of 128, bf16: 552 MB in
+// 106 us, 5.2 TB/s, about what a kernel that only reads reaches), otherwise the chain of loads that a workgroup begins with
+// (group, lengths, page, K, V) and the second launch: 7 us for 4 beams behind 300 keys.  Against one pass per sequence, which
+// reads shared keys once a beam: 16 x 8 beams behind 4,096 keys, heads of 128, 50 us and 167, heads of 64, 29 and 79.
 #include <type_traits>
 
 #include "common.h"
@@ -433,8 +440,8 @@ __device__ __forceinline__ float wave_of(float v, bool sum) {
 }
 
 // The cuts' sums and accumulators of a row at the largest of their references.  A wave takes a row, or with PARTS waves each
-// every so many of its cuts (32 cuts of 256 rows: 6.4 us a wave a row, 4.6 four).  Lanes: four elements each, of up to four cuts
-// side by side.
+// every so many of its cuts (the whole pass, bf16, heads of 64, a wave and four: 2 x 8 beams behind 9,000 keys in 38 cuts 10.4 and
+// 9.6 us, 3 x 4 behind 1,500 in 8 cuts, fp32, 10.3 and 11.1).  Lanes: four elements each, of up to four cuts side by side.
 template <typename T, int PARTS>
 __global__ __launch_bounds__(THREADS) void attn_beams_join_kernel(const float* acc, const float2* ml, T* __restrict__ out,
                                                                   const float* sinks, Args a) {

@@ -1762,9 +1762,11 @@ def _attn_beams_held(bf16: int, head_dim: int, block_size: int, rows: int) -> tu
 def attn_beams_cuts(q: torch.Tensor, k_pages: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, num_groups: int,
                     num_seqs: int, widest: int, max_shared: int, max_own: int) -> tuple[int, int]:
     """(cuts of the keys that a group shares, cuts of a sequence's own keys) for ``attn_beams``.  Own keys: up to eight waves a
-    compute unit, each with ``ATTN_BEAMS_OWN_KEYS``.  Shared ones: as many workgroups as the chip holds beside those of the
-    own keys, for what does not find room at once starts only when others end (2 x 8,192 shared keys of 4 beams, heads of 128:
-    12 cuts 20.0 us, 30 that fit 18.8, 32 that do not 22.2), each with a round of its waves at least (two in fp32).
+    compute unit, each with ``ATTN_BEAMS_OWN_KEYS``.  Shared ones: three eighths of the workgroups that the chip holds, each with
+    a round of its waves at least (two in fp32).  Few long cuts read as fast as many and leave the join less to do, yet they have
+    to keep every compute unit busy, also where groups are of uneven lengths (bf16, us, with an eighth, three eighths, as many as
+    fit beside the own keys' and all: heads of 128, 2 x 4 beams behind 8,192 keys 25.4, 17.1, 17.8, 20.4 and 4 x 8 behind 32,768
+    206, 106, 104, 106; heads of 64, 8 x 5 behind up to 2,900 20.9, 12.4, 12.4, 12.6 and 2 x 8 behind 9,000 9.8, 9.6, 10.8, 10.8).
     ``max_shared``, ``max_own``: the most shared keys of a group and own keys of a sequence (any cuts give right results for
     any lengths)."""
     units = compute_units(q.device)
@@ -1777,8 +1779,7 @@ def attn_beams_cuts(q: torch.Tensor, k_pages: torch.Tensor, num_heads: int, num_
     own = cuts(8 * units, num_seqs * num_kv_heads, max_own, ATTN_BEAMS_OWN_KEYS)
     if not num_groups or max_shared <= 0:
         return 0, own
-    room = held * units - -(-num_seqs * num_kv_heads * own // 4)
-    return cuts(room, num_groups * num_kv_heads * -(-rows // (16 * tiles)), max_shared,
+    return cuts(held * units * 3 // 8, num_groups * num_kv_heads * -(-rows // (16 * tiles)), max_shared,
                 ATTN_BEAMS_ROUND if q.dtype == BF16 else 2 * ATTN_BEAMS_ROUND), own
 
 
@@ -2916,7 +2917,7 @@ _BEAM_SELECT_ARGS = [c_int, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p] 
 
 def _beam_pieces(rows: int, vocab: int, count: int, device) -> tuple[int, int]:
     """(pieces of a row, logits of a piece): large pieces from a workgroup for every fourth compute unit on (small against
-    large: 4 rows of 8,192 logits 10.3 and 11.4 us, 4 of 128,256 12.6 and 11.8, 32 of 128,256 20.2 and 13.6)."""
+    large: 4 rows of 8,192 logits 8.1 and 8.9 us, 4 of 128,256 10.8 and 9.5, 32 of 128,256 15.6 and 10.8)."""
     small, large = BEAM_PIECES
     most = vocab + 7           # a row may begin inside its first 16 bytes
     piece = large if count <= 32 and 4 * rows * -(-most // large) >= compute_units(device) else small

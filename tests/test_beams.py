@@ -130,7 +130,7 @@ def test_cuts_fit_the_chip_and_the_keys(launched):
     cuts = lambda *a: ops.attn_beams_cuts(q, k, 32, 8, 64, *a)
     assert cuts(1, 4, 4, 300, 20) == (3, 1)                 # a round of the waves each
     assert cuts(0, 4, 1, 0, 1000) == (0, 16) and cuts(2, 4, 4, 0, 1) == (0, 1)
-    assert cuts(4, 16, 4, 100000, 20) == (15, 1)            # 512 workgroups less 32 over 32 items
+    assert cuts(4, 16, 4, 100000, 20) == (6, 1)             # three eighths of 512 workgroups over 32 items
     assert cuts(100, 400, 4, 100000, 300) == (1, 1)
     assert all(1 <= c <= 64 for n in (1, 7, 300) for c in cuts(n, 4 * n, 4, 10**6, 10**6))
 

@@ -405,7 +405,7 @@ __global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 
       const int g = min(g0 + lane, a.n_groups - 1);
       const unsigned long long here = __ballot(t.cu_groups[g] <= seq && seq < t.cu_groups[g + 1]);
       if (here) {
-        if (a.cs) lo = max(t.shared_lens[min(g0 + __ffsll(static_cast<long long>(here)) - 1, a.n_groups - 1)], 0);
+        if (a.cs) lo = min(max(t.shared_lens[min(g0 + __ffsll(static_cast<long long>(here)) - 1, a.n_groups - 1)], 0), most);
         grouped = true;
       }
     }
@@ -512,26 +512,24 @@ template <typename T> constexpr int TWO_TILES = sizeof(T) == 2 ? 128 : 64;
 int row_tiles_of(int bf16, int d, int bs, int rows) { return rows > 16 && d <= (bf16 ? TWO_TILES<bf16_t> : TWO_TILES<float>) && bs % 8 == 0 ? 2 : 1; }
 
 template <typename T, int DT, int RT, Form FORM>
-int launch(const Tensors<T>& t, const Args& a, int* per_cu, hipStream_t stream) {
-  if (per_cu)      // asked how many workgroups a compute unit holds
-    return static_cast<int>(hipOccupancyMaxActiveBlocksPerMultiprocessor(per_cu, attn_beams_kernel<T, DT, RT, FORM>, THREADS, 0));
+int launch(const Tensors<T>& t, const Args& a, hipStream_t stream) {
   const long items = static_cast<long>(a.n_groups) * a.cs * a.blocks * a.KV + (static_cast<long>(a.n_seqs) * a.co * a.KV + WAVES - 1) / WAVES;
   if (items * WAVES > 0x7fffffffL) return static_cast<int>(hipErrorInvalidValue);
   attn_beams_kernel<T, DT, RT, FORM><<<dim3(static_cast<unsigned>(items)), THREADS, 0, stream>>>(t, a);
   return kvf_last_error();
 }
-template <typename T, int DT> int launch_form(const Tensors<T>& t, const Args& a, int row_tiles, int* per_cu, hipStream_t stream) {
-  if (a.bs % 8) return launch<T, DT, 1, ANY>(t, a, per_cu, stream);
+template <typename T, int DT> int launch_form(const Tensors<T>& t, const Args& a, int row_tiles, hipStream_t stream) {
+  if (a.bs % 8) return launch<T, DT, 1, ANY>(t, a, stream);
   if constexpr (DT <= TWO_TILES<T> / 16)
-    if (row_tiles == 2) return a.d == DT * 16 ? launch<T, DT, 2, WHOLE>(t, a, per_cu, stream) : launch<T, DT, 2, ALIGNED>(t, a, per_cu, stream);
-  return a.d == DT * 16 ? launch<T, DT, 1, WHOLE>(t, a, per_cu, stream) : launch<T, DT, 1, ALIGNED>(t, a, per_cu, stream);
+    if (row_tiles == 2) return a.d == DT * 16 ? launch<T, DT, 2, WHOLE>(t, a, stream) : launch<T, DT, 2, ALIGNED>(t, a, stream);
+  return a.d == DT * 16 ? launch<T, DT, 1, WHOLE>(t, a, stream) : launch<T, DT, 1, ALIGNED>(t, a, stream);
 }
-template <typename T> int launch_dims(const Tensors<T>& t, const Args& a, int row_tiles, int* per_cu, hipStream_t stream) {
-  if (a.d <= 32) return launch_form<T, 2>(t, a, row_tiles, per_cu, stream);
-  if (a.d <= 64) return launch_form<T, 4>(t, a, row_tiles, per_cu, stream);
-  if (a.d <= 96) return launch_form<T, 6>(t, a, row_tiles, per_cu, stream);
-  if (a.d <= 128) return launch_form<T, 8>(t, a, row_tiles, per_cu, stream);
-  return launch_form<T, 16>(t, a, row_tiles, per_cu, stream);
+template <typename T> int launch_dims(const Tensors<T>& t, const Args& a, int row_tiles, hipStream_t stream) {
+  if (a.d <= 32) return launch_form<T, 2>(t, a, row_tiles, stream);
+  if (a.d <= 64) return launch_form<T, 4>(t, a, row_tiles, stream);
+  if (a.d <= 96) return launch_form<T, 6>(t, a, row_tiles, stream);
+  if (a.d <= 128) return launch_form<T, 8>(t, a, row_tiles, stream);
+  return launch_form<T, 16>(t, a, row_tiles, stream);
 }
 constexpr int JOIN_WIDE = 16;     // more cuts of a row than so many are joined by four waves
 
@@ -540,7 +538,7 @@ int run(const void* q, const void* k, const void* v, const int* table, const int
         void* out, float* acc, void* ml, const float* sinks, const Args& a, int row_tiles, hipStream_t stream) {
   const Tensors<T> t{static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), table, cu_groups, shared_lens, ctx_lens,
                      acc, static_cast<float2*>(ml)};
-  const int rc = launch_dims<T>(t, a, row_tiles, nullptr, stream);
+  const int rc = launch_dims<T>(t, a, row_tiles, stream);
   if (rc) return rc;
   const long rows = static_cast<long>(a.n_seqs) * a.H;
   if (a.cs + a.co > JOIN_WIDE && rows <= 0x7fffffffL / THREADS)
@@ -554,17 +552,6 @@ int run(const void* q, const void* k, const void* v, const int* table, const int
 // Tiles of 16 rows that a workgroup takes where a group has `rows` rows a kv head.
 KVF_EXPORT int kvf_attn_beams_row_tiles(int bf16, int d, int bs, int rows) { return row_tiles_of(bf16, d, bs, rows); }
 
-// Workgroups that a compute unit holds of the kernel that such heads take (0: it cannot be said).
-KVF_EXPORT int kvf_attn_beams_blocks_per_cu(int bf16, int d, int bs, int rows) {
-  if (d < 16 || d > 256 || d % 16 || bs < 1) return 0;
-  Args a{};
-  a.d = d;
-  a.bs = bs;
-  int n = 0;
-  const int rc = bf16 ? launch_dims<bf16_t>({}, a, row_tiles_of(1, d, bs, rows), &n, nullptr) : launch_dims<float>({}, a, row_tiles_of(0, d, bs, rows), &n, nullptr);
-  return rc ? 0 : n;
-}
-
 // q [n_seqs] rows of H heads; pages k [nb, KV, bs, d], v [nb, KV, d, bs]; table [n_seqs, width]; cu_groups [n_groups + 1];
 // shared_lens [n_groups]; ctx_lens [n_seqs].  Workspace: acc [n_seqs, H, cs + co, d], ml [n_seqs, H, cs + co, 2].
 KVF_EXPORT int kvf_attn_beams(int bf16, const void* q, const void* k, const void* v, const int* table, const int* cu_groups,
@@ -577,7 +564,7 @@ KVF_EXPORT int kvf_attn_beams(int bf16, const void* q, const void* k, const void
   if (static_cast<long>(width) * bs >= 1L << 30 || static_cast<long>(width) * bs * bs >= (1L << 32)) return static_cast<int>(hipErrorInvalidValue);
   if (n_seqs == 0) return 0;
   const long rows = static_cast<long>(widest) * (H / KV);
-  if (rows > 1 << 20) return static_cast<int>(hipErrorInvalidValue);
+  if (rows > 1 << 20 || static_cast<long>(n_seqs) * (H / KV) >= 1 << 22) return static_cast<int>(hipErrorInvalidValue);
   const int row_tiles = row_tiles_of(bf16, d, bs, static_cast<int>(rows)), blocks = static_cast<int>((rows + 16 * row_tiles - 1) / (16 * row_tiles));
   const Args a{H, KV, H / KV, d, bs, nb, width, q_stride, o_stride, n_seqs, n_groups, blocks, cs, co, scale * LOG2E, 1.f / static_cast<float>(H / KV),
                bs > 1 ? static_cast<unsigned>((1ull << 32) / bs) + 1u : 0u};

@@ -1752,35 +1752,37 @@ def attn_beams_takes(dtype: torch.dtype, head_dim: int) -> bool:
 
 
 @lru_cache(maxsize=None)
-def _attn_beams_held(bf16: int, head_dim: int, block_size: int, rows: int) -> tuple[int, int]:
-    """(tiles of 16 rows a workgroup takes, workgroups a compute unit holds) of the kernel for groups of ``rows`` rows a kv head."""
-    tiles = _fn("attn_beams", "kvf_attn_beams_row_tiles", [c_int] * 4)(bf16, head_dim, block_size, rows)
-    held = _fn("attn_beams", "kvf_attn_beams_blocks_per_cu", [c_int] * 4)(bf16, head_dim, block_size, rows)
-    return int(tiles), int(held) or 2
+def _attn_beams_tiles(bf16: int, head_dim: int, block_size: int, rows: int) -> int:
+    """Tiles of 16 rows that a workgroup takes where groups have ``rows`` rows a kv head."""
+    return int(_fn("attn_beams", "kvf_attn_beams_row_tiles", [c_int] * 4)(bf16, head_dim, block_size, rows))
 
 
 def attn_beams_cuts(q: torch.Tensor, k_pages: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, num_groups: int,
                     num_seqs: int, widest: int, max_shared: int, max_own: int) -> tuple[int, int]:
     """(cuts of the keys that a group shares, cuts of a sequence's own keys) for ``attn_beams``.  Own keys: up to eight waves a
-    compute unit, each with ``ATTN_BEAMS_OWN_KEYS``.  Shared ones: three eighths of the workgroups that the chip holds, each with
-    a round of its waves at least (two in fp32).  Few long cuts read as fast as many and leave the join less to do, yet they have
-    to keep every compute unit busy, also where groups are of uneven lengths (bf16, us, with an eighth, three eighths, as many as
-    fit beside the own keys' and all: heads of 128, 2 x 4 beams behind 8,192 keys 25.4, 17.1, 17.8, 20.4 and 4 x 8 behind 32,768
-    206, 106, 104, 106; heads of 64, 8 x 5 behind up to 2,900 20.9, 12.4, 12.4, 12.6 and 2 x 8 behind 9,000 9.8, 9.6, 10.8, 10.8).
-    ``max_shared``, ``max_own``: the most shared keys of a group and own keys of a sequence (any cuts give right results for
-    any lengths)."""
+    compute unit, each with ``ATTN_BEAMS_OWN_KEYS``.  Shared ones, each with a round of a workgroup's waves at least (two in fp32):
+    one workgroup a compute unit where it has two tiles of rows; for one tile, which asks for less between its loads, three for
+    four units (or one each, if that makes two cuts of one).  Further workgroups share units and leave the join more to do.
+    Measured, us, with half, three quarters, one, twice that of the compute units: one tile, 2 x 4 beams behind 8,192 keys
+    (heads of 128, bf16) 17.9, 17.1, 18.8, 20.8, 8 x 4 behind 2,048 (64, fp32) 20.0, 18.4, 20.0, 21.5; two, 4 x 8 behind 32,768
+    (128, bf16) 124, 106, 104, 106, 8 x 8 behind 4,096 (64, fp32) 47, 38, 32, 33, 8 x 5 behind up to 2,900 (64, bf16) 14.9, 13.7,
+    12.6, 12.7.  ``max_shared``, ``max_own``: the most shared keys of a group and own keys of a sequence (any cuts give right
+    results for any lengths)."""
     units = compute_units(q.device)
     rows = max(1, widest) * (num_heads // num_kv_heads)
-    tiles, held = _attn_beams_held(_tcode(q.dtype), head_dim, k_pages.shape[2], rows)
 
-    def cuts(room: int, items: int, keys: int, per: int) -> int:
-        return max(1, min(room // max(items, 1), -(-keys // per), ATTN_BEAMS_MAX_CUTS))
+    def cuts(most: int, keys: int, per: int) -> int:
+        return max(1, min(most, -(-keys // per), ATTN_BEAMS_MAX_CUTS))
 
-    own = cuts(8 * units, num_seqs * num_kv_heads, max_own, ATTN_BEAMS_OWN_KEYS)
+    own = cuts(8 * units // max(num_seqs * num_kv_heads, 1), max_own, ATTN_BEAMS_OWN_KEYS)
     if not num_groups or max_shared <= 0:
         return 0, own
-    return cuts(held * units * 3 // 8, num_groups * num_kv_heads * -(-rows // (16 * tiles)), max_shared,
-                ATTN_BEAMS_ROUND if q.dtype == BF16 else 2 * ATTN_BEAMS_ROUND), own
+    tiles = _attn_beams_tiles(_tcode(q.dtype), head_dim, k_pages.shape[2], rows)
+    items = num_groups * num_kv_heads * -(-rows // (16 * tiles))
+    most = units // items
+    if tiles == 1:
+        most = max(min(2, most), 3 * units // 4 // items)
+    return cuts(most, max_shared, ATTN_BEAMS_ROUND if q.dtype == BF16 else 2 * ATTN_BEAMS_ROUND), own
 
 
 def attn_beams_workspace(num_seqs: int, num_heads: int, head_dim: int, cuts: tuple[int, int], device
@@ -1797,9 +1799,9 @@ def attn_beams(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     """Attention of one token per sequence (row ``i`` of ``q`` is sequence ``i``'s) over ``ctx_lens[i]`` cached keys, for
     sequences in groups ``cu_groups[g] .. cu_groups[g + 1] - 1`` whose first ``shared_lens[g]`` keys are the same, as the beams
     of a request have them behind its prompt: these are read once for the whole group, from the pages of its first
-    sequence that holds as many.  (One that is shorter than what its group shares is read by itself.)  A sequence without keys gets zeros; one that no group names shares nothing.  Page numbers outside the
-    pages stand for keys that are not there.  ``widest``: sequences of the largest group (it decides how workgroups are laid out,
-    results do not depend on it).  ``cuts`` from ``attn_beams_cuts``, ``workspace`` from ``attn_beams_workspace``; launches that
+    sequence that holds as many.  (One that is shorter than what its group shares is read by itself.)  A sequence without keys
+    gets zeros; one that no group names shares nothing.  Page numbers outside the pages, and keys behind the table's end, are
+    not there.  ``widest``: sequences of the largest group (it decides how workgroups are laid out, results do not depend on it).  ``cuts`` from ``attn_beams_cuts``, ``workspace`` from ``attn_beams_workspace``; launches that
     share a workspace must not overlap.  ``sinks``: as in ``attn_prefill``.  Pages of any number of tokens (multiples of 8 are
     loaded widely), heads of up to 256 elements in steps of 16."""
     H, KV, d = num_heads, num_kv_heads, head_dim
@@ -1812,6 +1814,8 @@ def attn_beams(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     size = q.element_size()
     if q.shape[1] < H * d or q.stride(1) != 1 or (n > 1 and q.stride(0) * size % 16) or q.data_ptr() % 16:
         raise KernelError("attn_beams: rows of q hold all query heads, are dense and start on 16 bytes")
+    if n * (H // KV) >= 1 << 22 or q.stride(0) >= 1 << 31:
+        raise KernelError(f"attn_beams: {n} sequences of rows {q.stride(0)} apart are more than the kernel counts")
     _check(k_pages, "k_pages", q.dtype, (None, KV, None, d))
     nb, _, bs, _ = k_pages.shape
     _check(v_pages, "v_pages", q.dtype, (nb, KV, d, bs))
@@ -2936,9 +2940,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, cu_beams: torch.Tens
                 out_beams: torch.Tensor, out_tokens: torch.Tensor, workspace: tuple[torch.Tensor, ...]) -> None:
     """The best continuations of every request: of all its beams (rows ``cu_beams[r] .. cu_beams[r + 1] - 1`` of ``logits``, fp32
     or bf16) and tokens, the ``out_scores.shape[1]`` with the largest ``scores[beam] + log_softmax(logits[beam])[token]``, best
-    first (compared in 64 bits), equal ones by the lower beam, then the larger logit, then the lower token.  ``out_beams`` counts from the request's first beam.  Beams whose
-    score is not finite have ended and give none; tokens whose logit is NaN or -inf are ruled out (``+inf`` counts as the
-    largest finite number).  Where there are fewer candidates, the rest is (-inf, -1, -1).  ``workspace`` from
+    first (compared in 64 bits), equal ones by the lower beam, then the larger logit, then the lower token.  ``out_beams`` counts
+    from the request's first beam.  Beams whose score is not finite have ended and give none; tokens whose logit is NaN or -inf
+    are ruled out (``+inf`` counts as the largest finite number).  Where there are fewer candidates, the rest is (-inf, -1, -1).  ``workspace`` from
     ``beam_select_workspace``; launches that share one must not overlap."""
     if logits.dtype not in (F32, BF16):
         raise KernelError(f"beam_select takes float32 or bfloat16 logits, got {logits.dtype}")

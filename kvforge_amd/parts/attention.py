@@ -421,8 +421,8 @@ class PagedAttention(Mixer):
     def _reads_shared(self, shared) -> bool:
         """Whether the keys that sequences share (``SharedShape``) are read once a group: plain scores over all keys (and
         this class's own order of work)."""
-        return (shared is not None and type(self).forward is PagedAttention.forward and not (self.window or self.chunk) and self.slopes is None and not self.score_cap
-                and self.dist is None and self.score_slopes is None and self.distance_bias is None and self.d <= 256
+        return (shared is not None and type(self).forward is PagedAttention.forward and not (self.window or self.chunk)
+                and self.slopes is None and not self.score_cap and self.dist is None and self.score_slopes is None and self.distance_bias is None and self.d <= 256
                 and shared.max_shared > (0 if ops.plain_of(self.w_qkv).dtype == torch.float32 else SHARED_FROM))
 
     def launch_key(self, shape):

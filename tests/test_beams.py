@@ -38,12 +38,12 @@ def launched(monkeypatch):
     def fn(module, name, argtypes):
         def call(*args):
             made.append(name)
-            return {"kvf_beam_tile_bytes": 4096, "kvf_attn_beams_row_tiles": 1, "kvf_attn_beams_blocks_per_cu": 2}.get(name, 0)
+            return 4096 if name == "kvf_beam_tile_bytes" else 1 + (args[3] > 16) if name == "kvf_attn_beams_row_tiles" else 0
         return call
     monkeypatch.setattr(ops, "_fn", fn)
-    ops._attn_beams_held.cache_clear()
+    ops._attn_beams_tiles.cache_clear()
     yield made
-    ops._attn_beams_held.cache_clear()
+    ops._attn_beams_tiles.cache_clear()
 
 
 def select_args(rows=6, vocab=40, requests=2, count=4, dtype=F32):
@@ -125,12 +125,23 @@ def test_attention_refuses_what_its_kernels_do_not_take(launched):
     assert launched.count("kvf_attn_beams") == 2
 
 
+def test_attention_refuses_more_sequences_and_wider_strides_than_it_counts(launched):
+    ops.attn_beams(**attend_args(n=2, dtype=BF16))
+    apart = torch.empty(2**31 + 128, dtype=BF16).as_strided((2, 128), (2**31, 1))        # (nothing of it is touched)
+    many = torch.empty(2**21, 4 * 16, dtype=BF16)
+    for change in (dict(q=apart), dict(q=many, head_dim=16)):
+        with pytest.raises(ops.KernelError, match="more than the kernel counts"):
+            ops.attn_beams(**{**attend_args(n=2, dtype=BF16), **change})
+    assert launched.count("kvf_attn_beams") == 1
+
+
 def test_cuts_fit_the_chip_and_the_keys(launched):
     q, k = torch.zeros(1, 4, dtype=BF16), torch.zeros(1, 8, 16, 64, dtype=BF16)
     cuts = lambda *a: ops.attn_beams_cuts(q, k, 32, 8, 64, *a)
     assert cuts(1, 4, 4, 300, 20) == (3, 1)                 # a round of the waves each
     assert cuts(0, 4, 1, 0, 1000) == (0, 16) and cuts(2, 4, 4, 0, 1) == (0, 1)
-    assert cuts(4, 16, 4, 100000, 20) == (6, 1)             # three eighths of 512 workgroups over 32 items
+    assert cuts(4, 16, 4, 100000, 20) == (6, 1) and cuts(16, 64, 4, 100000, 20) == (2, 1)       # 32 and 128 items of one tile
+    assert cuts(4, 32, 8, 100000, 20) == (8, 1) and cuts(16, 128, 8, 100000, 20) == (2, 1)      # and of two
     assert cuts(100, 400, 4, 100000, 300) == (1, 1)
     assert all(1 <= c <= 64 for n in (1, 7, 300) for c in cuts(n, 4 * n, 4, 10**6, 10**6))
 

@@ -308,6 +308,18 @@ def test_attention_over_pages_of_any_size_in_any_cuts(dtype, page, cuts):
     check_attend(out, q, k, v, tables, ctx, 6, 2, 48, 0.2)
 
 
+@pytest.mark.parametrize("shared", [0, 16, 32, 48])
+def test_keys_behind_the_end_of_the_table_are_not_there(shared):
+    """Also where the group is said to share them: every key counts once, as the sinks in the denominators show."""
+    H, KV, d = 4, 2, 32
+    k, v, tables, cu, _, ctx = paged([(32, [40, 33, 32])], KV, d, 16, F32, 3)
+    q = torch.randn(len(ctx), H * d, generator=torch.Generator().manual_seed(6))
+    sinks = torch.tensor([0.5, 2.0, -1.0, 1.0])
+    short = [row[:2] for row in tables]
+    out = run_attend(q, k, v, short, cu, [shared], ctx, H, KV, d, 0.3, sinks)
+    check_attend(out, q, k, v, short, [32] * 3, H, KV, d, 0.3, sinks)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_shared_lengths_inside_a_page_and_beyond_a_sequence(dtype):
     """Any number of first keys may be shared, the table rows of a group agreeing on them; a sequence that is shorter is read

@@ -2990,29 +2990,36 @@ class CacheRows:
         if not self.tensors:
             raise KernelError("CacheRows: at least one tensor")
         first = self.tensors[0]
-        spans, tiles = [], []
+        many, device = first.shape[0] if first.dim() else 0, first.device
         tile_bytes = int(_fn("beam", "kvf_beam_tile_bytes", [])())
+        spans = []                  # (address, bytes from row to row, bytes of a row, address behind the last, unit)
         for t in self.tensors:
             _check(t, "tensor", None, None, contiguous=False)
-            if t.dim() < 2 or t.shape[0] != first.shape[0] or t.device != first.device or t.numel() == 0:
+            if t.dim() < 2 or t.shape[0] != many or t.device != device or t.numel() == 0:
                 raise KernelError("CacheRows: tensors [rows, ...] with as many rows, on one device")
-            size, row = t.element_size(), t[0].numel() * t.element_size()
-            stride = t.stride(0) * size if t.shape[0] > 1 else row
-            if not t[0].is_contiguous() or stride < row or size % 2:
+            size, elements, dense = t.element_size(), 1, True
+            for n, step in zip(t.shape[:0:-1], t.stride()[:0:-1]):
+                dense &= n == 1 or step == elements
+                elements *= n
+            row, at = elements * size, t.data_ptr()
+            stride = t.stride(0) * size if many > 1 else row
+            if not dense or stride < row or size % 2:
                 raise KernelError("CacheRows: rows are dense, do not overlap, and have elements of two bytes or more")
-            at = t.data_ptr()
-            behind = (t.shape[0] - 1) * stride
-            for a, s, b in spans:
-                if (a < at + behind + row and at < a + (t.shape[0] - 1) * s + b
-                        and (s != stride or (at - a) % s < b or (a - at) % s < row)):
-                    raise KernelError("CacheRows: rows of different tensors share memory")
-            spans.append((at, stride, row))
-            unit = next(u for u in (16, 8, 4, 2) if at % u == 0 and stride % u == 0 and row % u == 0)
-            from_ = torch.arange(0, row, tile_bytes, dtype=torch.int64)
-            tiles.append(torch.stack([from_ + at, torch.full_like(from_, stride),
-                                      (row - from_).clamp(max=tile_bytes) + (unit << 32)], dim=1))
-        self.rows, self.device = int(first.shape[0]), first.device
-        self.tiles = torch.cat(tiles).to(self.device)
+            together = at | stride | row
+            spans.append((at, stride, row, at + (many - 1) * stride + row, next(u for u in (16, 8, 4, 2) if together % u == 0)))
+        spanned: list[tuple] = []    # those that reach behind the address come to
+        for at, stride, row, end, _ in sorted(spans):
+            spanned = [s for s in spanned if s[3] > at]
+            if any(other != stride or (at - a) % other < held or (a - at) % other < row for a, other, held, *_ in spanned):
+                raise KernelError("CacheRows: rows of different tensors share memory")
+            spanned.append((at, stride, row, end))
+        at, stride, row, _, unit = torch.tensor(spans, dtype=torch.int64).T
+        counts = (row + (tile_bytes - 1)) // tile_bytes
+        of = torch.repeat_interleave(torch.arange(len(spans)), counts)
+        inside = (torch.arange(len(of)) - (counts.cumsum(0) - counts)[of]) * tile_bytes
+        tiles = torch.stack([at[of] + inside, stride[of], (row[of] - inside).clamp(max=tile_bytes) + (unit[of] << 32)], dim=1)
+        self.rows, self.device = int(many), device
+        self.tiles = tiles.to(device)
 
 
 def beam_reorder(rows: CacheRows, slots: torch.Tensor, parents: torch.Tensor) -> None:

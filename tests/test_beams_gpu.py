@@ -149,6 +149,15 @@ def test_selection_of_rows_that_begin_anywhere(dtype, offset):
     check_select(logits, scores, [0, 2, 5], 6, run_select(logits, scores, [0, 2, 5], 6))
 
 
+def test_selection_of_rows_behind_two_to_the_32():
+    """Offsets that pass 32 bits."""
+    held = torch.empty(2 * (2**31 + 8) + 3000, dtype=BF16, device=DEV)
+    logits = held.as_strided((3, 3000), (2**31 + 8, 1))
+    logits.copy_(torch.randn(3, 3000, generator=torch.Generator().manual_seed(1)) * 3)
+    scores = torch.tensor([-1.0, -0.5, -0.7], device=DEV)
+    check_select(logits, scores, [0, 3], 6, run_select(logits, scores, [0, 3], 6))
+
+
 def test_selection_tells_scores_of_beams_apart_that_32_bits_do_not():
     """Two beams whose best candidates differ by 2^-30 near 40: the order is the 64-bit one."""
     vocab = 4096
@@ -376,6 +385,22 @@ def test_pages_that_are_not_there_and_sequences_outside_groups(dtype):
     far = [c + 10**6 for c in ctx]
     out = run_attend(q, k.nan_to_num(1.0), v.nan_to_num(2.0), tables, cu, shared, far, H, KV, d, 0.3, cuts=(2, 2))
     check_attend(out, q, k.nan_to_num(1.0), v.nan_to_num(2.0), tables, far, H, KV, d, 0.3)
+
+
+@pytest.mark.parametrize("page", [16, 12])
+def test_pages_behind_two_to_the_32(page):
+    """Offsets that pass 32 bits: the pages of a small cache at the end of a large one."""
+    H, KV, d = 8, 2, 64
+    k, v, tables, cu, shared, ctx = paged([(48, [60, 100, 49]), (0, [30])], KV, d, page, BF16, 8)
+    first = 2**32 // (KV * page * d) + 5
+    far = [torch.empty(first + t.shape[0], *t.shape[1:], dtype=BF16, device=DEV) for t in (k, v)]
+    for held, t in zip(far, (k, v)):
+        held[0] = math.nan
+        held[first:].copy_(t)
+    q = torch.randn(len(ctx), H * d, generator=torch.Generator().manual_seed(4)).to(BF16)
+    moved = [[first + p if p >= 0 else p for p in row] for row in tables]
+    out = run_attend(q, *far, moved, cu, shared, ctx, H, KV, d, 0.2)
+    check_attend(out, q, k, v, tables, ctx, H, KV, d, 0.2)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

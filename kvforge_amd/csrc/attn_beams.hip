@@ -24,7 +24,7 @@
 // What bounds it: the keys' bytes where there are many of them (4 x 8 beams behind 32,768 keys, 8 kv heads of 128, bf16: 552 MB in
 // 106 us, 5.2 TB/s, about what a kernel that only reads reaches), otherwise the chain of loads that a workgroup begins with
 // (group, lengths, page, K, V) and the second launch: 7 us for 4 beams behind 300 keys.  Against one pass per sequence, which
-// reads shared keys once a beam: 16 x 8 beams behind 4,096 keys, heads of 128, 50 us and 167, heads of 64, 29 and 79.
+// reads shared keys once a beam: 16 x 8 beams behind 4,096 keys, heads of 128, 47 us and 167, heads of 64, 27 and 79.
 #include <type_traits>
 
 #include "common.h"

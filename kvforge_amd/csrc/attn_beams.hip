@@ -37,7 +37,8 @@ constexpr int BLOCK = 32;              // keys a wave takes at a time
 constexpr float LAZY = 8.f;
 constexpr float LOG2E = 1.4426950408889634f;
 
-// Where two waves a SIMD are asked for, a wave has at most 256 registers.
+// Where two waves a SIMD are asked for, a wave has at most 256 registers.  (fp32 heads of 128 need a few more: 12 x 16 beams
+// behind 1,777 keys, 24 heads, 106 us with spills, 95 with one wave a SIMD; heads of 64 in two tiles fit, 63 and 64.)
 #define KVF_TWO_WAVES(FITS) __attribute__((amdgpu_waves_per_eu((FITS) ? 2 : 1)))
 
 struct Args {
@@ -328,7 +329,7 @@ __device__ __forceinline__ void cut_of(int& lo, int& hi, int c, int n, int round
 // each in turn; of the others every wave takes a cut of a sequence's own keys by itself.  The kv head is the fastest index:
 // workgroups go to the eight XCDs in turn, so with eight heads an L2 holds the keys of one, also for a group's further rows.
 template <typename T, int DT, int RT, Form FORM>
-__global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 16 && DT < 16 : RT * DT <= 8) void attn_beams_kernel(Tensors<T> t, Args a) {
+__global__ __launch_bounds__(THREADS) KVF_TWO_WAVES(sizeof(T) == 2 ? RT * DT <= 16 && DT < 16 : RT * DT <= 8 && DT < 8) void attn_beams_kernel(Tensors<T> t, Args a) {
   __shared__ f32x4 lds_acc[RT][DT][WAVES - 1][KVF_WAVE];
   __shared__ float2 lds_ml[RT][WAVES][16];
   const int shared_items = a.n_groups * a.cs * a.blocks * a.KV;

@@ -1760,7 +1760,7 @@ def _attn_beams_tiles(bf16: int, head_dim: int, block_size: int, rows: int) -> i
 def attn_beams_cuts(q: torch.Tensor, k_pages: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, num_groups: int,
                     num_seqs: int, widest: int, max_shared: int, max_own: int) -> tuple[int, int]:
     """(cuts of the keys that a group shares, cuts of a sequence's own keys) for ``attn_beams``.  Own keys: up to eight waves a
-    compute unit, each with ``ATTN_BEAMS_OWN_KEYS``.  Shared ones, each with a round of a workgroup's waves at least (two in fp32):
+    compute unit, each with ``ATTN_BEAMS_OWN_KEYS``.  Shared ones, each with a round of a workgroup's waves at least:
     one workgroup a compute unit where it has two tiles of rows; for one tile, which asks for less between its loads, three for
     four units (or one each, if that makes two cuts of one).  Further workgroups share units and leave the join more to do.
     Measured, us, with half, three quarters, one, twice that of the compute units: one tile, 2 x 4 beams behind 8,192 keys
@@ -1782,7 +1782,7 @@ def attn_beams_cuts(q: torch.Tensor, k_pages: torch.Tensor, num_heads: int, num_
     most = units // items
     if tiles == 1:
         most = max(min(2, most), 3 * units // 4 // items)
-    return cuts(most, max_shared, ATTN_BEAMS_ROUND if q.dtype == BF16 else 2 * ATTN_BEAMS_ROUND), own
+    return cuts(most, max_shared, ATTN_BEAMS_ROUND), own
 
 
 def attn_beams_workspace(num_seqs: int, num_heads: int, head_dim: int, cuts: tuple[int, int], device

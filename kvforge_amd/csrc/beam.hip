@@ -696,39 +696,39 @@ __device__ __forceinline__ void loads_arrived() {
   asm volatile("" ::: "memory");
 }
 
-// What bounds it: bytes, each row that moves read and written once.  32 requests of 8 beams, 64 tensors of 32 KB rows: 349 MB in
-// 78 us from memory, 4.5 TB/s, as much as a plain copy of that size; 8 of 4 beams, 8 tensors of 1 MB rows: 160 MB in 44 us.
-// More bytes a lane do not help (tiles a workgroup U = 1, 2, 4, 8 for four beams: 43.8, 43.9, 46.2, 47.8 us): waves do.
-// A tile of all rows of a request: a lane's bytes of every row that moves are in its registers before it writes any of them, and
+// Tiles of all rows of a request: a lane's bytes of every row that moves are in its registers before it writes any of them, and
 // no other lane touches them, so rows may change places in any way (swaps and rings too) without memory beside them.
-// U whole tiles, 16 bytes at a time:
-template <int W, int U> __device__ __forceinline__ void move_whole(const Tile (&t)[U], const Moves<W>& m) {
-  Word4 v[W][U];
-  const int at = threadIdx.x * 16;
-#pragma unroll
-  for (int b = 0; b < W; ++b)
-    if (m.to[b] >= 0)
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[b][u] = get<Word4>(t[u].base + m.from[b] * t[u].stride, at);
-  loads_arrived();
-#pragma unroll
-  for (int b = 0; b < W; ++b)
-    if (m.to[b] >= 0)
-#pragma unroll
-      for (int u = 0; u < U; ++u) put(t[u].base + m.to[b] * t[u].stride, at, v[b][u]);
-}
-// any tile:
-template <typename Unit, int W> __device__ __forceinline__ void move_any(const Tile& t, const Moves<W>& m) {
-  constexpr int SIZE = sizeof(Unit);
-  for (int at = threadIdx.x * SIZE; at < t.bytes; at += THREADS * SIZE) {
-    Unit v[W];
+// What bounds it: bytes, each row that moves read and written once.  32 requests of 8 beams, 64 tensors of 32 KB rows: 349 MB in
+// 74 us from memory, 4.7 TB/s, as much as a plain copy of that size; 8 of 4 beams, 8 tensors of 1 MB rows: 160 MB in 37 us.
+// More bytes a lane do not help (tiles a workgroup U = 1, 2, 4, 8 for four beams: 43.8, 43.9, 46.2, 47.8 us): waves do.
+//
+// U tiles, a unit at a time; WHOLE: all of them are.  Units below 16 bytes lie THREADS apart, so that a lane has as many of them
+// in flight as registers for 16 bytes hold (tensors of 4-byte units: 12 us with one at a time, 15 requests of 13 beams).
+template <typename Unit, int W, int U, bool WHOLE> __device__ __forceinline__ void move_tiles(const Tile (&t)[U], const Moves<W>& m) {
+  constexpr int SIZE = sizeof(Unit), PASSES = TILE_BYTES / (THREADS * SIZE), PER = PASSES < 4 ? PASSES : 4;
+#pragma unroll 1
+  for (int pass = 0; pass < PASSES; pass += PER) {
+    Unit v[W][U][PER];
+    auto place = [&](int p) { return ((pass + p) * THREADS + static_cast<int>(threadIdx.x)) * SIZE; };
 #pragma unroll
     for (int b = 0; b < W; ++b)
-      if (m.to[b] >= 0) v[b] = get<Unit>(t.base + m.from[b] * t.stride, at);
+      if (m.to[b] >= 0)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int p = 0; p < PER; ++p) {
+            const int at = WHOLE ? place(p) : max(min(place(p), t[u].bytes - SIZE), 0);
+            v[b][u][p] = get<Unit>(t[u].base + m.from[b] * t[u].stride, at);
+          }
     loads_arrived();
 #pragma unroll
     for (int b = 0; b < W; ++b)
-      if (m.to[b] >= 0) put(t.base + m.to[b] * t.stride, at, v[b]);
+      if (m.to[b] >= 0)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int p = 0; p < PER; ++p)
+            if (WHOLE || place(p) < t[u].bytes) put(t[u].base + m.to[b] * t[u].stride, place(p), v[b][u][p]);
   }
 }
 
@@ -737,25 +737,26 @@ __global__ __launch_bounds__(THREADS) void beam_reorder_kernel(const Tile* __res
                                                                const int* __restrict__ slots, const int* __restrict__ parents) {
   Tile t[U];
   bool whole = true;
+  int unit = 16;                // that all of them can be moved by
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int i = blockIdx.x * U + u;
     t[u] = tiles[min(i, n_tiles - 1)];
-    whole &= i < n_tiles && t[u].unit == 16 && t[u].bytes == TILE_BYTES;
+    unit = min(unit, t[u].unit);
+    if (i >= n_tiles) t[u].bytes = 0;
+    whole &= t[u].bytes == TILE_BYTES;
   }
   Moves<W> m;
   m.read(slots + static_cast<size_t>(blockIdx.y) * beams, parents + static_cast<size_t>(blockIdx.y) * beams, beams, rows);
-  if (whole) {
-    move_whole<W, U>(t, m);
-    return;
-  }
-#pragma unroll 1
-  for (int i = blockIdx.x * U; i < min(static_cast<int>(blockIdx.x) * U + U, n_tiles); ++i) {
-    const Tile one = tiles[i];
-    if (one.unit == 16) move_any<Word4, W>(one, m);
-    else if (one.unit == 8) move_any<Word2, W>(one, m);
-    else if (one.unit == 4) move_any<uint32_t, W>(one, m);
-    else move_any<uint16_t, W>(one, m);
+  if (unit == 16) {
+    if (whole) move_tiles<Word4, W, U, true>(t, m);
+    else move_tiles<Word4, W, U, false>(t, m);
+  } else if (unit == 8) {
+    move_tiles<Word2, W, U, false>(t, m);
+  } else if (unit == 4) {
+    move_tiles<uint32_t, W, U, false>(t, m);
+  } else {
+    move_tiles<uint16_t, W, U, false>(t, m);
   }
 }
 

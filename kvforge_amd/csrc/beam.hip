@@ -617,28 +617,26 @@ int pieces_launch(const void* logits, const float* scores, double2* sums, float*
 }  // namespace
 
 // logits [rows][stride] of `vocab` (bf16: 0 fp32, 1 bf16); scores [rows]; cu_beams [requests + 1]; out_* [requests][count].
-// Workspace: sums [rows][pieces][2] in 64 bits, values/tokens [rows][pieces][count].  piece: elements of a piece, 256 times 8, or
-// 32 for up to 32 candidates.
+// Workspace: sums [rows][pieces][2] in 64 bits, values/tokens [rows][pieces][count].  piece: elements of a piece, 256 times 8,
+// 16, or 32 for up to 32 candidates.
 KVF_EXPORT int kvf_beam_select(int bf16, const void* logits, long stride, int rows, int vocab, const float* scores,
                                const int* cu_beams, int requests, int count, int pieces, int piece, void* sums,
                                float* values, int* tokens, float* out_scores, int* out_beams, int* out_tokens, hipStream_t stream) {
   if (count < 1 || count > MAX_COUNT || rows < 0 || rows > 65535 || vocab < 1 || pieces < 1 || requests < 0 ||
       static_cast<long>(pieces) * count > 65536)
     return static_cast<int>(hipErrorInvalidValue);
-  if (piece != THREADS * 8 && (piece != THREADS * 32 || count > 32)) return static_cast<int>(hipErrorInvalidValue);
+  if (piece != THREADS * 8 && piece != THREADS * 16 && (piece != THREADS * 32 || count > 32)) return static_cast<int>(hipErrorInvalidValue);
   if (requests == 0) return 0;
   // a row may begin up to 15 bytes into its first chunk
   if (static_cast<long>(pieces) * piece < static_cast<long>(vocab) + (bf16 ? 7 : 3)) return static_cast<int>(hipErrorInvalidValue);
   auto* sum = static_cast<double2*>(sums);
   if (rows) {
     const PieceArgs a{stride, rows, vocab, count, pieces, piece};
-    int rc;
-    if (bf16)
-      rc = piece == THREADS * 8 ? pieces_launch<bf16_t, 8>(logits, scores, sum, values, tokens, a, stream)
-                                : pieces_launch<bf16_t, 32>(logits, scores, sum, values, tokens, a, stream);
-    else
-      rc = piece == THREADS * 8 ? pieces_launch<float, 8>(logits, scores, sum, values, tokens, a, stream)
-                                : pieces_launch<float, 32>(logits, scores, sum, values, tokens, a, stream);
+#define KVF_PIECES(T) (piece == THREADS * 8    ? pieces_launch<T, 8>(logits, scores, sum, values, tokens, a, stream)   \
+                       : piece == THREADS * 16 ? pieces_launch<T, 16>(logits, scores, sum, values, tokens, a, stream)  \
+                                               : pieces_launch<T, 32>(logits, scores, sum, values, tokens, a, stream))
+    const int rc = bf16 ? KVF_PIECES(bf16_t) : KVF_PIECES(float);
+#undef KVF_PIECES
     if (rc) return rc;
   }
   const BestArgs b{rows, requests, count, pieces};

@@ -2914,18 +2914,22 @@ def decode_advance(sampled: torch.Tensor, token_ids: torch.Tensor, positions: to
 # ------------------------------------------------------------------------------ beam search
 BEAM_MAX_COUNT = 64      # candidates of a request
 BEAM_MAX_WIDTH = 32      # beams of a request that are reordered together
-BEAM_PIECES = (2048, 8192)     # logits of a row that one workgroup takes
+BEAM_PIECES = (2048, 4096, 8192)     # logits of a row that one workgroup takes
 _BEAM_REORDER_ARGS = [c_void_p] + [c_int] * 4 + [c_void_p] * 3
 _BEAM_SELECT_ARGS = [c_int, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 7
 
 
 def _beam_pieces(rows: int, vocab: int, count: int, device) -> tuple[int, int]:
-    """(pieces of a row, logits of a piece): large pieces from a workgroup for every fourth compute unit on (small against
-    large: 4 rows of 8,192 logits 8.1 and 8.9 us, 4 of 128,256 10.8 and 9.5, 32 of 128,256 15.6 and 10.8)."""
-    small, large = BEAM_PIECES
+    """(pieces of a row, logits of a piece): the smallest pieces that make fewer than four workgroups a compute unit and leave
+    the second kernel few enough candidates (four a lane, for half as many beams as candidates).  Us, with pieces of 2,048, 4,096
+    and 8,192: 4 rows of 8,192 logits, 8 best 8.3, 8.7, 9.2; 4 of 128,256 11.0, 9.2, 9.8, 32 of them 15.6, 11.6, 10.9; 13 of
+    16,034, 26 best 13.8, 11.4, 12.4; 154 of 3,858, 30 best, 13.4, 14.0, 14.8; 256 of 8,192, 8 best 10.4, 9.9, 10.5."""
     most = vocab + 7           # a row may begin inside its first 16 bytes
-    piece = large if count <= 32 and 4 * rows * -(-most // large) >= compute_units(device) else small
-    return -(-most // piece), piece
+    for piece in BEAM_PIECES if count <= 32 else BEAM_PIECES[:2]:
+        pieces = -(-most // piece)
+        if rows * pieces < 4 * compute_units(device) and -(-count // 16) * -(-pieces * count // 64) <= 4:
+            break
+    return pieces, piece
 
 
 def beam_select_workspace(rows: int, vocab: int, count: int, device) -> tuple[torch.Tensor, ...]:

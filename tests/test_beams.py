@@ -73,7 +73,7 @@ def test_selection_refuses_what_its_kernels_do_not_take(launched):
         ops.beam_select(**{**good, "logits": torch.zeros(1, 40).expand(70000, 40)})
     with pytest.raises(ops.KernelError, match="more than the kernel counts"):
         big = select_args(rows=1, vocab=40, requests=1, count=64)
-        ops.beam_select(**{**big, "logits": torch.zeros(1, 2048 * 1025, dtype=BF16), "cu_beams": torch.tensor([0, 1], dtype=I32)})
+        ops.beam_select(**{**big, "logits": torch.zeros(1, 4096 * 1025, dtype=BF16), "cu_beams": torch.tensor([0, 1], dtype=I32)})
     assert len(launched) == 2
 
 

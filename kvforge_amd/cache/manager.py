@@ -255,8 +255,9 @@ class CacheManager:
         self._next_serial += 1
 
     def shared_pages(self, request_ids: "list[str]", known: int = 0) -> int:
-        """How many entries at the start of the requests' tables are the same in all of them and every group without a window
-        (``known``: so many are)."""
+        """How many entries at the start of the requests' tables are the same in all of them and every group without a window.
+        ``known``: so many are, and are not compared; only pages that are filled stay the same (the last one of a table that
+        is being filled is replaced in every branch)."""
         n = None
         for g, group in enumerate(self.groups):
             if group.window is not None:

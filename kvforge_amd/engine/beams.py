@@ -254,7 +254,7 @@ class BeamSearcher:
         cache, bs = self.cache, self.cache.block_size
         width = batch[0].params.width
         logits = self._read_prompts(batch, ids)
-        common = [0] * len(batch)           # pages that all living beams of a search share
+        common = [0] * len(batch)           # filled pages that all living beams of a search, and so their descendants, share
         living = list(range(len(batch)))
         while True:
             searches = [batch[r] for r in living]
@@ -274,11 +274,12 @@ class BeamSearcher:
                 s = batch[r]
                 pos = len(s.prompt) + s.length - 1
                 here = [ids[r][p] for p in s.places]
-                common[r] = cache.shared_pages(here, common[r])
+                # (of one beam alone even the page that it fills is "shared", until it branches)
+                common[r] = min(cache.shared_pages(here, common[r]), pos // bs)
                 for p, rid in zip(s.places, here):
                     cache.append_slots(rid, pos + 1, pos)
                     entries.append(StepEntry(rid, [s.tokens[p][-1]], pos, "last"))
-                shared.append((len(here), min(common[r] * bs, pos)))
+                shared.append((len(here), common[r] * bs))
             logits = self.runner.step(entries, shared=shared)
             for e in entries:
                 cache.release_behind(e.request_id, e.start_pos + 1)

@@ -5,7 +5,7 @@
 //   S + (l - m) - log(sum_t exp(l_t - m)),   m = max_t l_t,
 // and the `count` best of a request are wanted, best first, equal scores by the lower beam, then the lower token.
 // Logits that are NaN or -inf are no candidates and weigh nothing, +inf counts as the largest finite number, and
-// beams whose score is not finite are passed over unread.
+// beams whose score is not finite are passed over unread.  Tokens that the caller rules out are no candidates either, but weigh.
 //
 //   1. `beam_pieces_kernel`: a workgroup takes a piece of a row, which stays in its registers (E logits a lane), so the row is
 //      read once.  Maximum, sum of exponentials, and the piece's `count` best, sorted.  They are found by a bound: the 64 largest logits of a wave's
@@ -133,13 +133,15 @@ __host__ __device__ __forceinline__ int list_room(int count, int e) { return ((c
 struct PieceArgs {
   long stride;          // elements from one row of logits to the next
   int rows, vocab, count, pieces, piece;   // `piece`: elements of a piece, a multiple of THREADS * Chunk::N
+  int n_ruled;          // tokens that are ruled out
 };
 
 // sums[row][piece] = (sum of exponentials, their reference), values/tokens[row][piece][count]: sorted, token -1 behind the last.
-template <typename T, int E>
+// RULED: the sum is made first, from the same logits in the same order, then the tokens in `ruled` leave the registers.
+template <typename T, int E, bool RULED>
 __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restrict__ logits, const float* __restrict__ scores,
                                                               double2* __restrict__ sums, float* __restrict__ values,
-                                                              int* __restrict__ tokens, PieceArgs a) {
+                                                              int* __restrict__ tokens, const int* __restrict__ ruled, PieceArgs a) {
   constexpr int N = Chunk<T>::N, CHUNKS = E / N;
   extern __shared__ __align__(16) unsigned long long list[];
   // list: (key, ~token) of what reaches the bound, a part for every wave
@@ -193,25 +195,63 @@ __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restric
     }
     mx = fminf(mx, LARGEST);
   }
+  float m = -INFINITY;
+  double s = 0.0;
+  auto sum_up = [&] {
+    if (m > -INFINITY) {
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        float part = 0.f;             // of neighbours; the lane's sum is 64 bits wide
+#pragma unroll
+        for (int i = 0; i < N; ++i) part += exp_unbiased(v[c][i] - m);
+        s += static_cast<double>(part);
+      }
+    }
+    s = wave_sum64(s);
+  };
+  if constexpr (RULED) {
+    const float wmx = wave_most(mx);
+    if (lane == 0) max_of[wave] = wmx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NWAVES; ++w) m = fmaxf(m, max_of[w]);
+    sum_up();
+    for (int k = 0; k < a.n_ruled; ++k) {
+      const int token = ruled[k];           // (the same for the whole workgroup)
+      if (token < lo || token < 0 || token >= hi) continue;
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (lo + (c * THREADS + tid) * N + i == token) v[c][i] = -INFINITY;
+    }
+    mx = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      top[c] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < N; ++i) top[c] = fmaxf(top[c], v[c][i]);
+      mx = fmaxf(mx, top[c]);
+    }
+  }
   const uint32_t lane_key = mx > -INFINITY ? order_key(mx) : 0u;
   uint32_t wave_bound, wave_share;
   kth_of_lanes(lane_key, a.count, (a.count + NWAVES - 1) / NWAVES, wave_bound, wave_share);
-  const float wmx = wave_most(mx);
+  const float wmx = RULED ? 0.f : wave_most(mx);
   if (lane == 0) {
     bound_of[wave] = wave_bound;
     share_of[wave] = wave_share;
-    max_of[wave] = wmx;
+    if (!RULED) max_of[wave] = wmx;
   }
   __syncthreads();
   // `count` logits reach every wave's own bound, and the least of the waves' shares
   uint32_t bound = share_of[0];
-  float m = -INFINITY;
 #pragma unroll
   for (int w = 1; w < NWAVES; ++w) bound = share_of[w] < bound ? share_of[w] : bound;
 #pragma unroll
   for (int w = 0; w < NWAVES; ++w) {
     bound = bound_of[w] > bound ? bound_of[w] : bound;
-    m = fmaxf(m, max_of[w]);
+    if (!RULED) m = fmaxf(m, max_of[w]);
   }
   // What is ahead of the bound, and what equals it in the order of the tokens.  Without a bound everything finite is taken.
   const unsigned long long below = (1ull << lane) - 1ull;
@@ -254,17 +294,7 @@ __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restric
       }
     }
   }
-  double s = 0.0;
-  if (m > -INFINITY) {
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-      float part = 0.f;             // of neighbours; the lane's sum is 64 bits wide
-#pragma unroll
-      for (int i = 0; i < N; ++i) part += exp_unbiased(v[c][i] - m);
-      s += static_cast<double>(part);
-    }
-  }
-  s = wave_sum64(s);
+  if (!RULED) sum_up();
   if (lane < LIST_STEP) mine[held + lane] = 0ull;       // the list is read in steps
   if (lane == 0) {
     sum_of[wave] = s;
@@ -609,20 +639,26 @@ __global__ __launch_bounds__(BEST_THREADS) void beam_best_kernel(const float* sc
 }
 
 template <typename T, int E>
-int pieces_launch(const void* logits, const float* scores, double2* sums, float* values, int* tokens, const PieceArgs& a, hipStream_t stream) {
+int pieces_launch(const void* logits, const float* scores, double2* sums, float* values, int* tokens, const int* ruled, const PieceArgs& a,
+                  hipStream_t stream) {
   const size_t lds = static_cast<size_t>(NWAVES) * list_room(a.count, E) * sizeof(unsigned long long);
-  beam_pieces_kernel<T, E><<<dim3(a.pieces, a.rows), THREADS, lds, stream>>>(static_cast<const T*>(logits), scores, sums, values, tokens, a);
+  const dim3 grid(a.pieces, a.rows);
+  const T* x = static_cast<const T*>(logits);
+  if (a.n_ruled) beam_pieces_kernel<T, E, true><<<grid, THREADS, lds, stream>>>(x, scores, sums, values, tokens, ruled, a);
+  else beam_pieces_kernel<T, E, false><<<grid, THREADS, lds, stream>>>(x, scores, sums, values, tokens, ruled, a);
   return kvf_last_error();
 }
 }  // namespace
 
 // logits [rows][stride] of `vocab` (bf16: 0 fp32, 1 bf16); scores [rows]; cu_beams [requests + 1]; out_* [requests][count].
 // Workspace: sums [rows][pieces][2] in 64 bits, values/tokens [rows][pieces][count].  piece: elements of a piece, 256 times 8,
-// 16, or 32 for up to 32 candidates.
+// 16, or 32 for up to 32 candidates.  ruled [n_ruled]: tokens that are no candidates, in any order (others than the vocabulary's say
+// nothing).
 KVF_EXPORT int kvf_beam_select(int bf16, const void* logits, long stride, int rows, int vocab, const float* scores,
                                const int* cu_beams, int requests, int count, int pieces, int piece, void* sums,
-                               float* values, int* tokens, float* out_scores, int* out_beams, int* out_tokens, hipStream_t stream) {
-  if (count < 1 || count > MAX_COUNT || rows < 0 || rows > 65535 || vocab < 1 || pieces < 1 || requests < 0 ||
+                               float* values, int* tokens, float* out_scores, int* out_beams, int* out_tokens, const int* ruled,
+                               int n_ruled, hipStream_t stream) {
+  if (count < 1 || count > MAX_COUNT || n_ruled < 0 || rows < 0 || rows > 65535 || vocab < 1 || pieces < 1 || requests < 0 ||
       static_cast<long>(pieces) * count > 65536)
     return static_cast<int>(hipErrorInvalidValue);
   if (piece != THREADS * 8 && piece != THREADS * 16 && (piece != THREADS * 32 || count > 32)) return static_cast<int>(hipErrorInvalidValue);
@@ -631,10 +667,10 @@ KVF_EXPORT int kvf_beam_select(int bf16, const void* logits, long stride, int ro
   if (static_cast<long>(pieces) * piece < static_cast<long>(vocab) + (bf16 ? 7 : 3)) return static_cast<int>(hipErrorInvalidValue);
   auto* sum = static_cast<double2*>(sums);
   if (rows) {
-    const PieceArgs a{stride, rows, vocab, count, pieces, piece};
-#define KVF_PIECES(T) (piece == THREADS * 8    ? pieces_launch<T, 8>(logits, scores, sum, values, tokens, a, stream)   \
-                       : piece == THREADS * 16 ? pieces_launch<T, 16>(logits, scores, sum, values, tokens, a, stream)  \
-                                               : pieces_launch<T, 32>(logits, scores, sum, values, tokens, a, stream))
+    const PieceArgs a{stride, rows, vocab, count, pieces, piece, n_ruled};
+#define KVF_PIECES(T) (piece == THREADS * 8    ? pieces_launch<T, 8>(logits, scores, sum, values, tokens, ruled, a, stream)   \
+                       : piece == THREADS * 16 ? pieces_launch<T, 16>(logits, scores, sum, values, tokens, ruled, a, stream)  \
+                                               : pieces_launch<T, 32>(logits, scores, sum, values, tokens, ruled, a, stream))
     const int rc = bf16 ? KVF_PIECES(bf16_t) : KVF_PIECES(float);
 #undef KVF_PIECES
     if (rc) return rc;

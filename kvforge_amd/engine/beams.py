@@ -1,8 +1,9 @@
 """Beam search over the step function and the paged cache.
 
 A search keeps several continuations of a prompt, its beams, and each step of a batch of searches is: one forward over the
-newest token of every living beam, ``ops.beam_select`` over the logits (the best ``2 * width`` continuations of every request,
-of which at least ``width`` do not end), and the beams' memory following the choice.  Pages that a beam has filled are shared by
+newest token of every living beam, ``ops.beam_select`` over the logits (the best ``2 * width`` continuations of every request;
+with several stop tokens more than ``width`` of them may end, and the best of those that do not are selected by themselves where that
+happens), and the beams' memory following the choice.  Pages that a beam has filled are shared by
 its descendants (``CacheManager.branch``); the page that it is filling, and its state slots, are its own, and
 ``ops.beam_reorder`` copies them, in all layers with one launch a cache group.  A beam that goes on keeps its place (its
 request id, rows and pages) with the first of its descendants, so only what has several is copied, into places whose beams were
@@ -65,19 +66,22 @@ class Search:
         self.ended.sort(key=lambda s: -s.score)     # stable: of equals the first to end comes first
         del self.ended[self.params.width:]
 
-    def advance(self, candidates: "Sequence[tuple[float, int, int]]") -> dict[int, int]:
-        """Take the step's candidates (log-probability, number of the living beam, token), best first.  Returns the parent's place
-        of every living place; those whose beam goes on in its own place are their own parents."""
+    def lacks(self, candidates: "Sequence[tuple[float, int, int]]", asked: int) -> bool:
+        """Whether so many of the ``asked`` best candidates end that there may be others to go on with behind them."""
+        return len(candidates) >= asked and sum(token not in self.stops for _, _, token in candidates) < self.params.width
+
+    def advance(self, candidates: "Sequence[tuple[float, int, int]]",
+                going_on: "Sequence[tuple[float, int, int]] | None" = None) -> dict[int, int]:
+        """Take the step's candidates (log-probability, number of the living beam, token), best first, and, where they lack such,
+        the best of those that do not end.  Returns the parent's place of every living place; those whose beam goes on in its own
+        place are their own parents."""
         width = self.params.width
-        chosen: list[tuple[int, int, float]] = []
         self.length += 1
-        for rank, (log_prob, beam, token) in enumerate(candidates):
-            place = self.places[beam]
+        for log_prob, beam, token in candidates[:width]:        # what ends must be among the best itself
             if token in self.stops:
-                if rank < width:        # what ends must be among the best itself
-                    self._end(self.tokens[place] + [token], log_prob, FinishReason.STOP)
-            elif len(chosen) < width:
-                chosen.append((place, token, log_prob))
+                self._end(self.tokens[self.places[beam]] + [token], log_prob, FinishReason.STOP)
+        chosen = [(self.places[beam], token, log_prob) for log_prob, beam, token in (candidates if going_on is None else going_on)
+                  if token not in self.stops][:width]
         if self.length >= self.max_tokens:
             for place, token, log_prob in chosen:
                 self._end(self.tokens[place] + [token], log_prob, FinishReason.LENGTH)
@@ -122,7 +126,7 @@ class BeamSearcher:
         self._count = 0
 
     # ------------------------------------------------------------------ device work
-    def _select(self, logits: torch.Tensor, searches: "list[Search]", count: int):
+    def _select(self, logits: torch.Tensor, searches: "list[Search]", count: int, ruled_out: torch.Tensor | None = None):
         """Candidates of every search, best first, as lists of (log-probability, beam, token)."""
         rows, vocab = logits.shape
         requests = len(searches)
@@ -140,7 +144,8 @@ class BeamSearcher:
         flat[rows] = 0
         flat[rows + 1:] = np.cumsum([len(s.places) for s in searches])
         dev.copy_(host, non_blocking=True)
-        ops.beam_select(logits, dev[:rows].view(torch.float32), dev[rows:], out[0].view(torch.float32), out[1], out[2], work)
+        ops.beam_select(logits, dev[:rows].view(torch.float32), dev[rows:], out[0].view(torch.float32), out[1], out[2], work,
+                        ruled_out)
         got = out.cpu().numpy()             # waits: the staging memory is free again
         scores, beams, tokens = got[0].view(np.float32).tolist(), got[1].tolist(), got[2].tolist()
         return [[c for c in zip(*request) if c[1] >= 0] for request in zip(scores, beams, tokens)]
@@ -256,10 +261,19 @@ class BeamSearcher:
         logits = self._read_prompts(batch, ids)
         common = [0] * len(batch)           # filled pages that all living beams of a search, and so their descendants, share
         living = list(range(len(batch)))
+        ruled_out = None                    # the stop tokens, on the device (all searches have the same)
         while True:
             searches = [batch[r] for r in living]
             found = self._select(logits, searches, 2 * width)
-            parents = [s.advance(c) for s, c in zip(searches, found)]
+            going_on = [None] * len(searches)
+            lacking = [s.lacks(c, 2 * width) for s, c in zip(searches, found)]
+            if any(lacking):
+                if ruled_out is None:
+                    stops = [t for t in sorted(batch[0].stops) if 0 <= t < logits.shape[1]]
+                    ruled_out = torch.tensor(stops, dtype=torch.int32, device=self.device)
+                others = self._select(logits, searches, 2 * width, ruled_out)
+                going_on = [c if short else None for c, short in zip(others, lacking)]
+            parents = [s.advance(c, o) for s, c, o in zip(searches, found, going_on)]
             self._follow(searches, [ids[r] for r in living], parents, width)
             for r in living:
                 s = batch[r]

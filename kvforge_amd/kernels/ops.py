@@ -2916,7 +2916,7 @@ BEAM_MAX_COUNT = 64      # candidates of a request
 BEAM_MAX_WIDTH = 32      # beams of a request that are reordered together
 BEAM_PIECES = (2048, 4096, 8192)     # logits of a row that one workgroup takes
 _BEAM_REORDER_ARGS = [c_void_p] + [c_int] * 4 + [c_void_p] * 3
-_BEAM_SELECT_ARGS = [c_int, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 7
+_BEAM_SELECT_ARGS = [c_int, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p] * 7 + [c_int, c_void_p]
 
 
 def _beam_pieces(rows: int, vocab: int, count: int, device) -> tuple[int, int]:
@@ -2941,13 +2941,15 @@ def beam_select_workspace(rows: int, vocab: int, count: int, device) -> tuple[to
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, cu_beams: torch.Tensor, out_scores: torch.Tensor,
-                out_beams: torch.Tensor, out_tokens: torch.Tensor, workspace: tuple[torch.Tensor, ...]) -> None:
+                out_beams: torch.Tensor, out_tokens: torch.Tensor, workspace: tuple[torch.Tensor, ...],
+                ruled_out: torch.Tensor | None = None) -> None:
     """The best continuations of every request: of all its beams (rows ``cu_beams[r] .. cu_beams[r + 1] - 1`` of ``logits``, fp32
     or bf16) and tokens, the ``out_scores.shape[1]`` with the largest ``scores[beam] + log_softmax(logits[beam])[token]``, best
     first (compared in 64 bits), equal ones by the lower beam, then the larger logit, then the lower token.  ``out_beams`` counts
     from the request's first beam.  Beams whose score is not finite have ended and give none; tokens whose logit is NaN or -inf
-    are ruled out (``+inf`` counts as the largest finite number).  Where there are fewer candidates, the rest is (-inf, -1, -1).  ``workspace`` from
-    ``beam_select_workspace``; launches that share one must not overlap."""
+    are ruled out (``+inf`` counts as the largest finite number).  Where there are fewer candidates, the rest is (-inf, -1, -1).
+    ``ruled_out`` (int32): tokens that are no candidates of any beam but keep their weight, so that scores are those of a call
+    without it, to the bit.  ``workspace`` from ``beam_select_workspace``; launches that share one must not overlap."""
     if logits.dtype not in (F32, BF16):
         raise KernelError(f"beam_select takes float32 or bfloat16 logits, got {logits.dtype}")
     _check(logits, "logits", None, (None, None), contiguous=False)
@@ -2976,12 +2978,15 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, cu_beams: torch.Tens
     _check(tokens, "workspace[2]", I32, (None,))
     if (sums.shape[0] < rows * pieces * 2 or min(values.shape[0], tokens.shape[0]) < rows * pieces * count or sums.data_ptr() % 16):
         raise KernelError("beam_select: workspace too small for these rows, logits and candidates")
-    stream = _here("beam_select", (out_scores, out_beams, out_tokens, sums, values, tokens), (logits, scores, cu_beams))
+    if ruled_out is not None:
+        _check(ruled_out, "ruled_out", I32, (None,))
+    stream = _here("beam_select", (out_scores, out_beams, out_tokens, sums, values, tokens), (logits, scores, cu_beams, ruled_out))
     stride = logits.stride(0) if rows > 1 else vocab
     f = _fn("beam", "kvf_beam_select", _BEAM_SELECT_ARGS)
     _ok(f(_tcode(logits.dtype), logits.data_ptr(), stride, rows, vocab, scores.data_ptr(),
           cu_beams.data_ptr(), requests, count, pieces, piece, sums.data_ptr(), values.data_ptr(),
-          tokens.data_ptr(), out_scores.data_ptr(), out_beams.data_ptr(), out_tokens.data_ptr(), stream), "beam_select")
+          tokens.data_ptr(), out_scores.data_ptr(), out_beams.data_ptr(), out_tokens.data_ptr(),
+          ruled_out.data_ptr() if ruled_out is not None else None, ruled_out.shape[0] if ruled_out is not None else 0, stream), "beam_select")
 
 
 class CacheRows:

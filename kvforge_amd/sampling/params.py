@@ -35,7 +35,8 @@ class SamplingParams:
 @dataclass
 class BeamParams:
     """Parameters of a beam search.  ``width`` beams a request are followed, the best by the sum of their tokens' log-probabilities;
-    a beam whose next token is a stop token ends.  Ended beams are ranked by that sum over ``(number of output tokens) **
+    one whose next token is a stop token ends, if it is among the ``width`` best of all continuations, and the ``width`` best of the
+    others go on.  Ended beams are ranked by that sum over ``(number of output tokens) **
     length_penalty`` (the stop token counts).  A request is done once ``width`` beams have ended and, unless
     ``early_stopping``, no living beam's score so far beats the worst of them; or after ``max_tokens``, where the living ones
     end too.  ``num_return``: how many sequences are handed back, the best first (default: all ``width``)."""

@@ -14,7 +14,7 @@ from kvforge_amd.engine.beams import BeamSearcher
 from kvforge_amd.kernels import ops
 from kvforge_amd.parts import attention_pages
 from kvforge_amd.sampling.params import BeamParams
-from tests.plain import beams as plain
+from tests.plain import beam_search, beams as plain
 
 VOCAB, NONE = 13, -1
 
@@ -90,14 +90,20 @@ def select_by(keep=lambda turn, candidates: candidates):
     """Selection by its definition, of whose candidates (all there are of a request) ``keep`` leaves some."""
     turns = []
 
-    def select(logits, searches, count, *_):
+    def select(logits, searches, count, ruled_out=None):
+        if ruled_out is not None:
+            out = set(ruled_out.tolist())
+            return [[c for c in found if c[2] not in out][:count] for found in plain.select(logits, *rows_of(searches), VOCAB * 16)]
         turns.append(len(turns))
-        scores = torch.tensor([s.log_probs[p] for s in searches for p in s.places], dtype=torch.float64)
-        cu = [0]
-        for s in searches:
-            cu.append(cu[-1] + len(s.places))
-        return [keep(turns[-1], found)[:count] for found in plain.select(logits, scores, cu, VOCAB * 16)]
+        return [keep(turns[-1], found)[:count] for found in plain.select(logits, *rows_of(searches), VOCAB * 16)]
     return select
+
+
+def rows_of(searches):
+    cu = [0]
+    for s in searches:
+        cu.append(cu[-1] + len(s.places))
+    return torch.tensor([s.log_probs[p] for s in searches for p in s.places], dtype=torch.float64), cu
 
 
 def empty(cache):
@@ -137,3 +143,38 @@ def test_sharing_that_is_known_is_of_filled_pages():
     assert m.shared_pages(["a", "b"], known) == 1
     m.branch("b", "a", 9)
     assert m.shared_pages(["a", "b"], known) == m.shared_pages(["a", "b"]) == 2
+
+
+# ------------------------------------------------------------------------------------- several stop tokens
+@pytest.mark.parametrize("width,stops", [(1, (3, 8)), (2, (0, 5)), (2, (1, 4, 9)), (4, (0, 3, 6, 9)), (3, tuple(range(12))), (5, tuple(range(11))),
+                                         (4, tuple(range(0, 13, 2))), (2, tuple(range(13)))])
+@pytest.mark.parametrize("early,penalty", [(False, 1.0), (True, 1.0), (False, 0.0), (False, 2.0)])
+def test_searches_follow_as_many_beams_as_they_can_whatever_ends(on_the_cpu, width, stops, early, penalty):
+    """Against the definition, which looks at all continuations; at what ends, whatever that is, and at what goes on."""
+    for seed in range(6):
+        runner = PagedToy(seed)
+        runner.table[..., list(stops)] += 1.0            # what ends is likely
+        searcher = BeamSearcher(runner)
+        searcher._select = select_by()
+        params = BeamParams(width=width, max_tokens=9, length_penalty=penalty, early_stopping=early)
+        prompts = [[2, 7], [5, 1, 0, 4, 12]]
+        for prompt, found in zip(prompts, searcher.run(prompts, params, set(stops))):
+            want = beam_search.search(runner.after, prompt, width, 9, penalty, early, set(stops))
+            got = found.output().sequences
+            assert [(s.output_token_ids, s.finish_reason.value) for s in got] == [(t, r) for t, _, _, r in want]
+            assert all(abs(s.log_prob - p) < 1e-9 and abs(s.score - q) < 1e-9 for s, (_, p, q, _) in zip(got, want))
+        empty(runner.cache)
+
+
+def test_one_of_two_beams_is_looked_for_behind_what_ends():
+    from kvforge_amd.engine.beams import Search
+    s = Search([1], BeamParams(width=2, max_tokens=5), {8, 9}, 5)
+    assert s.advance([(-1.0, 0, 3), (-1.1, 0, 4), (-3.0, 0, 8), (-4.0, 0, 9)]) == {0: 0, 1: 0}
+    best = [(-1.2, 0, 5), (-1.3, 0, 9), (-1.4, 1, 9), (-1.5, 1, 8)]
+    assert s.lacks(best, 4) and not s.lacks(best[:3], 4) and not s.lacks([*best[:2], (-1.4, 1, 5), best[3]], 4)
+    assert s.advance(best, [best[0], (-4.0, 1, 0), (-4.1, 0, 0), (-4.2, 0, 1)]) == {0: 0, 1: 1}
+    assert s.tokens == {0: [3, 5], 1: [4, 0]} and [e.output_token_ids for e in s.ended] == [[3, 9]] and not s.done
+    # all of the best end: two have ended that no living one can pass
+    ends = [(-2.2, 0, 8), (-2.3, 0, 9), (-2.4, 0, 6), (-2.5, 1, 8)]
+    assert s.lacks(ends, 4)
+    assert s.advance(ends, [ends[2], (-5.0, 1, 0)]) == {} and s.done

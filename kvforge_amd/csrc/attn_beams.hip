@@ -2,7 +2,8 @@
 // pages (the beams of a request behind its prompt): the keys that a group shares are read once for all its rows.
 //
 //   out = softmax(scale * q K^T) V per head, over the keys [0, ctx) of the sequence; sinks: one more term exp(sink_h) in the
-//   denominator.  A sequence without keys gets zeros.
+//   denominator.  A sequence without keys gets zeros.  gate: every output is multiplied by sigmoid(gate), in fp32 ahead of its one
+//   rounding.
 //
 // A workgroup of four waves takes a cut of a range of keys for one kv head and up to 16 * RT rows: of the shared keys, rows are
 // (sequence of the group, head that shares the kv head); of a sequence's own keys, the heads alone.  Every cut leaves its
@@ -443,9 +444,9 @@ __device__ __forceinline__ float wave_of(float v, bool sum) {
 // The cuts' sums and accumulators of a row at the largest of their references.  A wave takes a row, or with PARTS waves each
 // every so many of its cuts (the whole pass, bf16, heads of 64, a wave and four: 2 x 8 beams behind 9,000 keys in 38 cuts 10.4 and
 // 9.6 us, 3 x 4 behind 1,500 in 8 cuts, fp32, 10.3 and 11.1).  Lanes: four elements each, of up to four cuts side by side.
-template <typename T, int PARTS>
+template <typename T, int PARTS, bool GATED>
 __global__ __launch_bounds__(THREADS) void attn_beams_join_kernel(const float* acc, const float2* ml, T* __restrict__ out,
-                                                                  const float* sinks, Args a) {
+                                                                  const float* sinks, const T* __restrict__ gate, int gate_stride, Args a) {
   __shared__ f32x4 lds[WAVES][KVF_WAVE];
   const int lane = threadIdx.x % KVF_WAVE, wave = threadIdx.x / KVF_WAVE, cuts = a.cs + a.co;
   const int part = wave % PARTS;
@@ -473,6 +474,10 @@ __global__ __launch_bounds__(THREADS) void attn_beams_join_kernel(const float* a
   };
   const int first = sub * PARTS + part;
   load(first);
+  f32x4 z = f32x4{0.f, 0.f, 0.f, 0.f};
+  if constexpr (GATED)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = Elem<T>::load(gate + row / a.H * gate_stride + static_cast<long>(h) * a.d + min(at, quads - 1) * 4 + i);
   const float2 none = make_float2(-INFINITY, 0.f);
   const float2 one = lane < cuts ? mine[lane] : none, two = lane + KVF_WAVE < cuts ? mine[lane + KVF_WAVE] : none;
   const float sink = sinks != nullptr ? sinks[h] * LOG2E : -INFINITY;
@@ -504,7 +509,10 @@ __global__ __launch_bounds__(THREADS) void attn_beams_join_kernel(const float* a
   if (sub == 0 && at < quads) {
     T* to = out + row / a.H * a.o_stride + static_cast<long>(h) * a.d + at * 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) Elem<T>::store(to + i, any ? o[i] / total : 0.f);
+    for (int i = 0; i < 4; ++i) {
+      const float x = any ? o[i] / total : 0.f;
+      Elem<T>::store(to + i, GATED ? x / (1.f + expf(-z[i])) : x);
+    }
   }
 }
 
@@ -536,16 +544,22 @@ constexpr int JOIN_WIDE = 16;     // more cuts of a row than so many are joined 
 
 template <typename T>
 int run(const void* q, const void* k, const void* v, const int* table, const int* cu_groups, const int* shared_lens, const int* ctx_lens,
-        void* out, float* acc, void* ml, const float* sinks, const Args& a, int row_tiles, hipStream_t stream) {
+        void* out, float* acc, void* ml, const float* sinks, const void* gate, int gate_stride, const Args& a, int row_tiles, hipStream_t stream) {
   const Tensors<T> t{static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), table, cu_groups, shared_lens, ctx_lens,
                      acc, static_cast<float2*>(ml)};
   const int rc = launch_dims<T>(t, a, row_tiles, stream);
   if (rc) return rc;
   const long rows = static_cast<long>(a.n_seqs) * a.H;
-  if (a.cs + a.co > JOIN_WIDE && rows <= 0x7fffffffL / THREADS)
-    attn_beams_join_kernel<T, WAVES><<<static_cast<unsigned>(rows), THREADS, 0, stream>>>(acc, static_cast<const float2*>(ml), static_cast<T*>(out), sinks, a);
-  else
-    attn_beams_join_kernel<T, 1><<<static_cast<unsigned>((rows + WAVES - 1) / WAVES), THREADS, 0, stream>>>(acc, static_cast<const float2*>(ml), static_cast<T*>(out), sinks, a);
+  auto join = [&](auto parts, auto gated, long groups) {
+    attn_beams_join_kernel<T, decltype(parts)::value, decltype(gated)::value><<<static_cast<unsigned>(groups), THREADS, 0, stream>>>(
+        acc, static_cast<const float2*>(ml), static_cast<T*>(out), sinks, static_cast<const T*>(gate), gate_stride, a);
+  };
+  auto join_rows = [&](auto gated) {
+    if (a.cs + a.co > JOIN_WIDE && rows <= 0x7fffffffL / THREADS) join(std::integral_constant<int, WAVES>{}, gated, rows);
+    else join(std::integral_constant<int, 1>{}, gated, (rows + WAVES - 1) / WAVES);
+  };
+  if (gate != nullptr) join_rows(std::true_type{});
+  else join_rows(std::false_type{});
   return kvf_last_error();
 }
 }  // namespace
@@ -554,21 +568,23 @@ int run(const void* q, const void* k, const void* v, const int* table, const int
 KVF_EXPORT int kvf_attn_beams_row_tiles(int bf16, int d, int bs, int rows) { return row_tiles_of(bf16, d, bs, rows); }
 
 // q [n_seqs] rows of H heads; pages k [nb, KV, bs, d], v [nb, KV, d, bs]; table [n_seqs, width]; cu_groups [n_groups + 1];
-// shared_lens [n_groups]; ctx_lens [n_seqs].  Workspace: acc [n_seqs, H, cs + co, d], ml [n_seqs, H, cs + co, 2].
+// shared_lens [n_groups]; ctx_lens [n_seqs]; gate: null, or [n_seqs] rows of H * d elements, gate_stride apart.  Workspace: acc [n_seqs, H, cs + co, d], ml [n_seqs, H, cs + co, 2].
 KVF_EXPORT int kvf_attn_beams(int bf16, const void* q, const void* k, const void* v, const int* table, const int* cu_groups,
-                              const int* shared_lens, const int* ctx_lens, void* out, float* acc, void* ml, const float* sinks, int H,
+                              const int* shared_lens, const int* ctx_lens, void* out, float* acc, void* ml, const float* sinks,
+                              const void* gate, int gate_stride, int H,
                               int KV, int d, int bs, int nb, int width, int q_stride, int o_stride, int n_seqs, int n_groups, int widest,
                               int cs, int co, float scale, hipStream_t stream) {
   if (KV < 1 || H < KV || H % KV || d < 16 || d > 256 || d % 16 || bs < 1 || nb < 1 || width < 0 || n_seqs < 0 || n_groups < 0 ||
       widest < 1 || cs < 0 || co < 1 || cs > 64 || co > 64 || (n_groups == 0 && cs))
     return static_cast<int>(hipErrorInvalidValue);
   if (static_cast<long>(width) * bs >= 1L << 30 || static_cast<long>(width) * bs * bs >= (1L << 32)) return static_cast<int>(hipErrorInvalidValue);
+  if (gate != nullptr && gate_stride < H * d && n_seqs > 1) return static_cast<int>(hipErrorInvalidValue);
   if (n_seqs == 0) return 0;
   const long rows = static_cast<long>(widest) * (H / KV);
   if (rows > 1 << 20 || static_cast<long>(n_seqs) * (H / KV) >= 1 << 22) return static_cast<int>(hipErrorInvalidValue);
   const int row_tiles = row_tiles_of(bf16, d, bs, static_cast<int>(rows)), blocks = static_cast<int>((rows + 16 * row_tiles - 1) / (16 * row_tiles));
   const Args a{H, KV, H / KV, d, bs, nb, width, q_stride, o_stride, n_seqs, n_groups, blocks, cs, co, scale * LOG2E, 1.f / static_cast<float>(H / KV),
                bs > 1 ? static_cast<unsigned>((1ull << 32) / bs) + 1u : 0u};
-  return bf16 ? run<bf16_t>(q, k, v, table, cu_groups, shared_lens, ctx_lens, out, acc, ml, sinks, a, row_tiles, stream)
-              : run<float>(q, k, v, table, cu_groups, shared_lens, ctx_lens, out, acc, ml, sinks, a, row_tiles, stream);
+  return bf16 ? run<bf16_t>(q, k, v, table, cu_groups, shared_lens, ctx_lens, out, acc, ml, sinks, gate, gate_stride, a, row_tiles, stream)
+              : run<float>(q, k, v, table, cu_groups, shared_lens, ctx_lens, out, acc, ml, sinks, gate, gate_stride, a, row_tiles, stream);
 }

@@ -1731,7 +1731,7 @@ def attn_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
 ATTN_BEAMS_MAX_CUTS = 64
 ATTN_BEAMS_ROUND = 128       # keys that the waves of a workgroup take at a time
 ATTN_BEAMS_OWN_KEYS = 64     # keys of a sequence's own that are worth a wave
-_ATTN_BEAMS_ARGS = [c_int] + [c_void_p] * 11 + [c_int] * 13 + [c_float, c_void_p]
+_ATTN_BEAMS_ARGS = [c_int] + [c_void_p] * 12 + [c_int] * 14 + [c_float, c_void_p]
 
 
 def _here(who: str, outs: tuple, ins: tuple) -> int:
@@ -1795,14 +1795,14 @@ def attn_beams_workspace(num_seqs: int, num_heads: int, head_dim: int, cuts: tup
 def attn_beams(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, cu_groups: torch.Tensor,
                shared_lens: torch.Tensor, ctx_lens: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_heads: int,
                head_dim: int, scale: float, widest: int, cuts: tuple[int, int], workspace: tuple[torch.Tensor, torch.Tensor],
-               sinks: torch.Tensor | None = None) -> None:
+               sinks: torch.Tensor | None = None, gate: torch.Tensor | None = None) -> None:
     """Attention of one token per sequence (row ``i`` of ``q`` is sequence ``i``'s) over ``ctx_lens[i]`` cached keys, for
     sequences in groups ``cu_groups[g] .. cu_groups[g + 1] - 1`` whose first ``shared_lens[g]`` keys are the same, as the beams
     of a request have them behind its prompt: these are read once for the whole group, from the pages of its first
     sequence that holds as many.  (One that is shorter than what its group shares is read by itself.)  A sequence without keys
     gets zeros; one that no group names shares nothing.  Page numbers outside the pages, and keys behind the table's end, are
     not there.  ``widest``: sequences of the largest group (it decides how workgroups are laid out, results do not depend on it).  ``cuts`` from ``attn_beams_cuts``, ``workspace`` from ``attn_beams_workspace``; launches that
-    share a workspace must not overlap.  ``sinks``: as in ``attn_prefill``.  Pages of any number of tokens (multiples of 8 are
+    share a workspace must not overlap.  ``sinks``, ``gate``: as in ``attn_prefill`` (a gate in 32 bits too).  Pages of any number of tokens (multiples of 8 are
     loaded widely), heads of up to 256 elements in steps of 16."""
     H, KV, d = num_heads, num_kv_heads, head_dim
     if KV < 1 or H < 1 or H % KV:
@@ -1848,10 +1848,15 @@ def attn_beams(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     if pa.shape[0] < n * H * (cs + co) * d or pm.shape[0] < n * H * (cs + co) * 2 or pa.data_ptr() % 16:
         raise KernelError("attn_beams: workspace too small")
     sk = _sinks_ptr(sinks, H, q)
-    stream = _here("attn_beams", (out, pa, pm), (q, k_pages, v_pages, block_table, cu_groups, shared_lens, ctx_lens, sinks))
+    gp, gs = None, 0
+    if gate is not None:
+        gp, gs = _gate_args(gate, q, H * d)
+        if gs >= 1 << 31:
+            raise KernelError(f"attn_beams: rows of the gate {gs} apart are more than the kernel counts")
+    stream = _here("attn_beams", (out, pa, pm), (q, k_pages, v_pages, block_table, cu_groups, shared_lens, ctx_lens, sinks, gate))
     f = _fn("attn_beams", "kvf_attn_beams", _ATTN_BEAMS_ARGS)
     _ok(f(_tcode(q.dtype), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), cu_groups.data_ptr(),
-          shared_lens.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), pa.data_ptr(), pm.data_ptr(), sk, H, KV, d, bs, nb, width,
+          shared_lens.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), pa.data_ptr(), pm.data_ptr(), sk, gp, gs, H, KV, d, bs, nb, width,
           q.stride(0) if n > 1 else H * d, H * d, n, groups, int(widest), cs, co, float(scale), stream), "attn_beams")
 
 

@@ -520,7 +520,7 @@ class PagedAttention(Mixer):
             out.append(((self.prefix, "head_gates"), x, self.w_head_gate, gates, "store"))
         return out
 
-    def _attend_shared(self, qkv, step, layer: LayerState, table, out, shared) -> None:
+    def _attend_shared(self, qkv, step, layer: LayerState, table, out, shared, gate) -> None:
         """Attention of single tokens whose sequences share pages."""
         H, KV, d, n, s = self.H, self.KV, self.d, step.n_seqs, shared.shape
         key = ("attention.shared_cuts", H, KV, d, qkv.dtype)
@@ -530,7 +530,7 @@ class PagedAttention(Mixer):
         parts = n * H * sum(cuts)
         workspace = (step.ws.buf("shared_part_acc", (parts * d,), torch.float32), step.ws.buf("shared_part_ml", (parts * 2,), torch.float32))
         ops.attn_beams(qkv, layer.k_pages, layer.v_pages, table, shared.cu_groups, shared.shared_lens, step.ctx_lens, out, H, KV, d,
-                       self.scale, s.widest, cuts, workspace, sinks=self.sinks)
+                       self.scale, s.widest, cuts, workspace, sinks=self.sinks, gate=gate)
 
     def forward(self, x, step, layer: LayerState, residual) -> None:
         """``x``: normalised activations, or (after ``absorb_norm``) the fp32 residual stream."""
@@ -618,7 +618,7 @@ class PagedAttention(Mixer):
         bs = layer.k_pages.shape[2]
         work, rows_per_item = self._prefill_work(step, act, bs)
         gate = qkv[:, g0:g0 + H * d] if self.gated else None
-        # the matrix-core kernels gate their output as they store it
+        # the matrix-core kernels, and those for shared pages, gate their output as they store it
         gate_in_kernel = gate if gate is not None and ops.attention_on_matrix_cores(act, bs, d) else None
         if work is not None:
             ops.attn_prefill(qkv, layer.k_pages, layer.v_pages, table, step.cu_q, step.ctx_lens,
@@ -627,8 +627,8 @@ class PagedAttention(Mixer):
                              score_cap=self.score_cap, chunk=chunk, dist=self.dist)
         shared = step.shared if step.shared is not None and self._reads_shared(step.shared.shape) else None
         if shared is not None:
-            gate_in_kernel = None
-            self._attend_shared(qkv, step, layer, table, out, shared)
+            gate_in_kernel = gate
+            self._attend_shared(qkv, step, layer, table, out, shared, gate)
         elif step.n_decode:
             splits, in_order = self._decode_plan(step, ops.attention_on_matrix_cores(act, bs, d))
             token_is_seq = step.decode_seq_ids is None and work is None

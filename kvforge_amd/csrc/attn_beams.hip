@@ -13,14 +13,15 @@
 //   S^T (keys x rows) = K Q^T in two tiles t of 16 keys; tile row i is key 8 (i / 4) + 4 t + i % 4, so that a lane ends up with
 //     the scores of the eight neighbouring keys 8 g .. 8 g + 7 of row r;
 //   O^T (d x rows) += V^T P^T: V pages hold an element's keys side by side, so a lane's eight keys of one element are one load,
-//     and its probabilities are the other operand as they stand (bf16: rounded once; fp32: v_mfma_f32_16x16x4_f32 takes them
+//     and its probabilities are the other operand as they stand (bf16: as two numbers; fp32: v_mfma_f32_16x16x4_f32 takes them
 //     key by key).
 // Fragments come from the pages in this order, nothing is staged.  Lanes without a valid page read page 0 and are masked.
 //
 // A row's reference (what is subtracted in the exponent) is raised only when a score passes it by LAZY (in log2 units); scores,
-// sums and accumulators are fp32.  bf16: a probability is rounded to bf16 on its way into the product with V, as the cached V is;
-// errors of different keys do not add up in one direction, and outputs are off by up to 0.0023 of their largest where rounding
-// them to bf16 alone costs 0.0017.  Two bf16 parts a probability would come down to that, for 4% of the time.
+// sums and accumulators are fp32.  bf16: a probability enters its product with V as the sum of two bf16 numbers, itself rounded and
+// what that leaves, 2^-16 of it off: outputs are off by the rounding of what is stored (0.0017 of their largest; rounded once,
+// probabilities alone would make that up to 0.0025).  The second products take 0.5 of 13.7 us where the chain of a few blocks bounds (8 x
+// up to 5 beams behind up to 2,900 keys), and 0.2% where the bytes do.
 //
 // What bounds it: the keys' bytes where there are many of them (4 x 8 beams behind 32,768 keys, 8 kv heads of 128, bf16: 552 MB in
 // 106 us, 5.2 TB/s, about what a kernel that only reads reaches), otherwise the chain of loads that a workgroup begins with
@@ -71,14 +72,20 @@ template <> struct Frag<bf16_t> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) k.v[i] = keep >> i & 1u ? k.v[i] : static_cast<__bf16>(0.f);
   }
-  struct Probs { bf16x8 v; };
+  struct Probs { bf16x8 v, rest; };     // v + rest
   static __device__ __forceinline__ Probs probs(const f32x4 (&p)[2]) {
     Probs o;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o.v[i] = static_cast<__bf16>(p[i / 4][i % 4]);
+    for (int i = 0; i < 8; ++i) {
+      o.v[i] = static_cast<__bf16>(p[i / 4][i % 4]);
+      o.rest[i] = static_cast<__bf16>(p[i / 4][i % 4] - static_cast<float>(o.v[i]));
+    }
     return o;
   }
-  static __device__ __forceinline__ f32x4 values(const Keys& k, const Probs& p, f32x4 acc) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(k.v, p.v, acc, 0, 0, 0); }
+  static __device__ __forceinline__ f32x4 values(const Keys& k, const Probs& p, f32x4 acc) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k.v, p.rest, acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(k.v, p.v, acc, 0, 0, 0);
+  }
 };
 template <> struct Frag<float> {
   static constexpr int SLICE = 16;

@@ -1,0 +1,44 @@
+"""bf16 attention behind shared pages is off by no more than its inputs' type asks: sums as exact as in 32 bits, and the one rounding of
+what is stored."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.plain import beams as plain
+from tests.test_beams_gpu import GROUPS, paged, run_attend
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def check(out, q, k, v, tables, ctx, H, KV, d, scale, sinks=None):
+    """A score is off by 2^-24 sqrt(d) of its size, a probability by as much: 2.5e-5 of the sum of |p v| (scores up to 8).  A probability
+    goes into its product as two bf16 numbers: the first is off by at most 2^-8 of it, the second by 2^-8 of that, 2^-16.  What
+    is stored is off by 2^-8 of itself."""
+    want, weight = plain.attend(q, k, v, tables, ctx, H, KV, d, scale, sinks)
+    inner = (2.5e-5 + 2.0 ** -16) * weight + 1e-7
+    off = (out.cpu().double() - want).abs()
+    bound = inner + 2.0 ** -8 * (want.abs() + inner)
+    assert bool((off <= bound).all()), float((off - bound).max())
+
+
+@pytest.mark.parametrize("groups", sorted(GROUPS))
+@pytest.mark.parametrize("H,KV,d", [(4, 2, 16), (6, 2, 80), (8, 2, 64), (3, 3, 128), (8, 1, 256), (40, 2, 32), (32, 2, 128), (24, 2, 96)])
+def test_bf16_outputs_are_rounded_once(groups, H, KV, d):
+    k, v, tables, cu, shared, ctx = paged(GROUPS[groups], KV, d, 16, BF16, 15)
+    q = (torch.randn(len(ctx), H * d, generator=torch.Generator().manual_seed(11)) * 1.3).to(BF16)
+    sinks = torch.randn(H, generator=torch.Generator().manual_seed(2)) if H == 8 else None
+    out = run_attend(q, k, v, tables, cu, shared, ctx, H, KV, d, d ** -0.5, sinks)
+    check(out, q, k, v, tables, ctx, H, KV, d, d ** -0.5, sinks)
+
+
+@pytest.mark.parametrize("page", [1, 3, 8, 12, 32])
+@pytest.mark.parametrize("cuts", [(1, 1), (64, 64)])
+def test_bf16_outputs_of_any_pages_and_cuts(page, cuts):
+    groups = [(96, [97, 130, 110]), (48, [48, 49]), (0, [200])]
+    k, v, tables, cu, shared, ctx = paged(groups, 2, 48, page, BF16, page + 1)
+    q = torch.randn(len(ctx), 6 * 48, generator=torch.Generator().manual_seed(page)).to(BF16)
+    out = run_attend(q, k, v, tables, cu, shared, ctx, 6, 2, 48, 0.2, cuts=cuts)
+    check(out, q, k, v, tables, ctx, 6, 2, 48, 0.2)

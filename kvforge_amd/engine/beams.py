@@ -200,18 +200,20 @@ class BeamSearcher:
             needs.append(self.pages_needed(len(prompt), params, most))
         if params.width > runner.meta.max_seqs:
             raise ValueError(f"{params.width} beams are more than the runner's {runner.meta.max_seqs} sequences")
+        # (a batch gives back what it held, so there is as much for each)
+        free = min((p.num_free for p in cache.pools), default=math.inf)
+        slots = cache.slots.num_free if cache.slots.num_slots else math.inf
+        for s, need in zip(searches, needs):        # ahead of all work
+            if need > free or params.width > slots:
+                raise ValueError(f"a search of {params.width} beams behind {len(s.prompt)} tokens needs {need} pages and {params.width} state "
+                                 f"slots, {free} pages and {slots} slots are free")
         at = 0
         while at < len(searches):
-            free = min((p.num_free for p in cache.pools), default=math.inf)
-            slots = cache.slots.num_free if cache.slots.num_slots else math.inf
             n = pages = 0
             while (at + n < len(searches) and (n + 1) * params.width <= min(runner.meta.max_seqs, slots)
                    and pages + needs[at + n] <= free):
                 pages += needs[at + n]
                 n += 1
-            if n == 0:
-                raise ValueError(f"a search of {params.width} beams behind {len(searches[at].prompt)} tokens needs {needs[at]} pages "
-                                 f"and {params.width} sequences, {free} pages are free")
             self._run_batch(searches[at:at + n])
             at += n
         return searches

@@ -178,3 +178,25 @@ def test_one_of_two_beams_is_looked_for_behind_what_ends():
     ends = [(-2.2, 0, 8), (-2.3, 0, 9), (-2.4, 0, 6), (-2.5, 1, 8)]
     assert s.lacks(ends, 4)
     assert s.advance(ends, [ends[2], (-5.0, 1, 0)]) == {} and s.done
+
+
+# ------------------------------------------------------------------------------------- searches that do not fit
+@pytest.mark.parametrize("kind", ["pages", "slots", "positions", "empty"])
+def test_a_list_of_prompts_is_refused_ahead_of_all_work(on_the_cpu, kind):
+    """The last of them is the one that does not fit."""
+    runner = PagedToy(blocks=16 if kind == "pages" else 120, seqs=3 if kind == "slots" else 16)
+    runner.meta.max_seqs = 16
+    searcher = BeamSearcher(runner)
+    searcher._select = select_by()
+    steps = []
+    step = runner.step
+    runner.step = lambda *a, **kw: (steps.append(1), step(*a, **kw))[1]
+    last = {"pages": [1] * 50, "slots": [1, 2, 3], "positions": [1] * 64, "empty": []}[kind]
+    params = BeamParams(width=4, max_tokens=5)
+    with pytest.raises(ValueError):
+        searcher.run([[1, 2], [3, 4, 5], last], params, set())
+    assert not steps
+    empty(runner.cache)
+    if kind != "slots":
+        assert all(s.done for s in searcher.run([[1, 2], [3, 4, 5]] * 3, params, set()))
+        empty(runner.cache)

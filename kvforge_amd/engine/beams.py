@@ -198,8 +198,10 @@ class BeamSearcher:
                                  f"{runner.max_model_len}")
             searches.append(Search(prompt, params, stops, most))
             needs.append(self.pages_needed(len(prompt), params, most))
-        if params.width > runner.meta.max_seqs:
-            raise ValueError(f"{params.width} beams are more than the runner's {runner.meta.max_seqs} sequences")
+        at_once = min(runner.meta.max_seqs, runner.meta.max_tokens)        # beams of a step, a token each
+        if params.width > at_once:
+            raise ValueError(f"{params.width} beams are more than the {at_once} that a step takes ({runner.meta.max_seqs} sequences, "
+                             f"{runner.meta.max_tokens} tokens)")
         # (a batch gives back what it held, so there is as much for each)
         free = min((p.num_free for p in cache.pools), default=math.inf)
         slots = cache.slots.num_free if cache.slots.num_slots else math.inf
@@ -210,7 +212,7 @@ class BeamSearcher:
         at = 0
         while at < len(searches):
             n = pages = 0
-            while (at + n < len(searches) and (n + 1) * params.width <= min(runner.meta.max_seqs, slots)
+            while (at + n < len(searches) and (n + 1) * params.width <= min(at_once, slots)
                    and pages + needs[at + n] <= free):
                 pages += needs[at + n]
                 n += 1

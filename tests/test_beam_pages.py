@@ -23,7 +23,7 @@ class PagedToy:
     """A runner whose model keeps a token's number in its page and in the request's slot, and whose logits go by the last two tokens
     that it finds there.  Steps with groups read the shared keys from the first sequence's pages."""
 
-    def __init__(self, seed=0, block=4, blocks=120, seqs=16, window=None) -> None:
+    def __init__(self, seed=0, block=4, blocks=120, seqs=16, window=None, tokens=9) -> None:
         groups = [CacheGroup((0,), attention_pages(1, 16))]
         if window:
             groups.append(CacheGroup((1,), attention_pages(1, 16), window=window))
@@ -32,7 +32,7 @@ class PagedToy:
         self.storage = SimpleNamespace(pages=self.pages)
         self.seen = torch.full((seqs, 64), NONE)
         self.states = SimpleNamespace(tensors={"seen": self.seen})
-        self.meta = SimpleNamespace(max_seqs=seqs, max_tokens=7)
+        self.meta = SimpleNamespace(max_seqs=seqs, max_tokens=tokens)
         self.model = SimpleNamespace(config=SimpleNamespace(vocab_size=VOCAB))
         self.max_model_len = 64
         self.table = torch.randn(VOCAB, VOCAB, VOCAB, generator=torch.Generator().manual_seed(seed)) * 2
@@ -47,6 +47,7 @@ class PagedToy:
 
     def step(self, entries, shared=None):
         cache, bs, logits = self.cache, self.cache.block_size, []
+        assert len(entries) <= self.meta.max_seqs and sum(len(e.token_ids) for e in entries) <= self.meta.max_tokens
         for e in entries:
             for j, t in enumerate(e.token_ids, e.start_pos):
                 for g in range(cache.num_groups):
@@ -200,3 +201,19 @@ def test_a_list_of_prompts_is_refused_ahead_of_all_work(on_the_cpu, kind):
     if kind != "slots":
         assert all(s.done for s in searcher.run([[1, 2], [3, 4, 5]] * 3, params, set()))
         empty(runner.cache)
+
+
+@pytest.mark.parametrize("seqs,tokens", [(16, 4), (16, 7), (16, 8), (4, 64), (9, 64)])
+def test_batches_keep_to_the_sequences_and_tokens_of_a_step(on_the_cpu, seqs, tokens):
+    runner = PagedToy(seqs=16, tokens=tokens)
+    runner.meta.max_seqs = seqs
+    searcher = BeamSearcher(runner)
+    searcher._select = select_by()
+    prompts = [[2, 7], [5, 1, 0, 4, 12], [3], [8, 8, 1, 2, 9, 10, 0, 4, 4, 4]]
+    for prompt, found in zip(prompts, searcher.run(prompts, BeamParams(width=4, max_tokens=5), {3})):
+        want = beam_search.search(runner.after, prompt, 4, 5, stops={3})
+        assert [s.output_token_ids for s in found.output().sequences] == [t for t, _, _, _ in want]
+    empty(runner.cache)
+    with pytest.raises(ValueError):
+        searcher.run(prompts, BeamParams(width=min(seqs, tokens) + 1, max_tokens=5), set())
+    empty(runner.cache)

@@ -57,7 +57,28 @@ def parse_args(argv: list[str] | None = None) -> argparse.Namespace:
     p.add_argument("--no-decode-run-ahead", action="store_true",
                    help="do not queue the next run of decode steps before the current one is read")
     p.add_argument("--json", action="store_true", help="print one JSON object instead of text")
-    return p.parse_args(argv)
+    args = p.parse_args(argv)
+    if args.beams is None:
+        if args.length_penalty != 1.0 or args.early_stopping:
+            p.error("--length-penalty and --early-stopping are a beam search's (--beams)")
+        return args
+    # a search draws nothing
+    if args.temperature != 0.0 or args.top_k != 0 or args.top_p != 1.0:
+        p.error("--beams searches: --temperature, --top-k and --top-p sample")
+    if args.model and args.seed != 0:
+        p.error("--beams searches: beside --model there is nothing that --seed could draw")
+    try:
+        _beam_params(args)
+    except ValueError as e:
+        p.error(str(e))
+    return args
+
+
+def _beam_params(args):
+    from kvforge_amd.sampling.params import BeamParams
+
+    return BeamParams(width=args.beams, max_tokens=args.max_tokens, length_penalty=args.length_penalty,
+                      early_stopping=args.early_stopping, ignore_eos=args.ignore_eos, stop_token_ids=_ids(args.stop_token_ids))
 
 
 def _ids(text: str) -> list[int]:
@@ -66,12 +87,7 @@ def _ids(text: str) -> list[int]:
 
 def _search(args, engine, name: str, prompts: list) -> int:
     """``--beams``: the prompts' best continuations."""
-    from kvforge_amd.sampling.params import BeamParams
-
-    params = BeamParams(width=args.beams, max_tokens=args.max_tokens, length_penalty=args.length_penalty,
-                        early_stopping=args.early_stopping, ignore_eos=args.ignore_eos,
-                        stop_token_ids=_ids(args.stop_token_ids))
-    outs = engine.beam_search(prompts, params)
+    outs = engine.beam_search(prompts, _beam_params(args))
     if args.json:
         print(json.dumps({"model": name, "outputs": [
             {"prompt_token_ids": o.prompt_token_ids, "sequences": [

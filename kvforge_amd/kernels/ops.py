@@ -2938,11 +2938,13 @@ def _beam_pieces(rows: int, vocab: int, count: int, device) -> tuple[int, int]:
 
 
 def beam_select_workspace(rows: int, vocab: int, count: int, device) -> tuple[torch.Tensor, ...]:
-    """Scratch of ``beam_select`` for ``rows`` rows of logits: the pieces' sums, their best logits and the tokens of these."""
-    pieces, _ = _beam_pieces(rows, vocab, count, device)
-    return (torch.empty(rows * pieces * 2, dtype=torch.float64, device=device),
-            torch.empty(rows * pieces * count, dtype=F32, device=device),
-            torch.empty(rows * pieces * count, dtype=I32, device=device))
+    """Scratch of ``beam_select`` for up to ``rows`` rows of ``vocab`` logits and ``count`` candidates: the pieces' sums, their best
+    logits and the tokens of these."""
+    pieces = rows * _beam_pieces(rows, vocab, count, device)[0]
+    # fewer rows may be cut more finely, as long as that makes fewer than four workgroups a compute unit
+    pieces = max(pieces, min(rows * -(-(vocab + 7) // BEAM_PIECES[0]), 4 * compute_units(device) - 1))
+    return (torch.empty(pieces * 2, dtype=torch.float64, device=device), torch.empty(pieces * count, dtype=F32, device=device),
+            torch.empty(pieces * count, dtype=I32, device=device))
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, cu_beams: torch.Tensor, out_scores: torch.Tensor,

@@ -18,8 +18,8 @@
 // Fragments come from the pages in this order, nothing is staged.  Lanes without a valid page read page 0 and are masked.
 //
 // A row's reference (what is subtracted in the exponent) is raised only when a score passes it by LAZY (in log2 units); scores,
-// sums and accumulators are fp32.  bf16: a probability enters its product with V as the sum of two bf16 numbers, itself rounded and
-// what that leaves, 2^-16 of it off: outputs are off by the rounding of what is stored (0.0017 of their largest; rounded once,
+// sums and accumulators are fp32.  bf16: a probability enters its product with V as the sum of two bf16 numbers, itself cut and
+// what that leaves, 2^-15 of it off: outputs are off by the rounding of what is stored (0.0017 of their largest; rounded once,
 // probabilities alone would make that up to 0.0025).  The second products take 0.5 of 13.7 us where the chain of a few blocks bounds (8 x
 // up to 5 beams behind up to 2,900 keys), and 0.2% where the bytes do.
 //
@@ -72,13 +72,16 @@ template <> struct Frag<bf16_t> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) k.v[i] = keep >> i & 1u ? k.v[i] : static_cast<__bf16>(0.f);
   }
-  struct Probs { bf16x8 v, rest; };     // v + rest
+  // v + rest, v the largest bf16 number below the probability: neither is zero where the probability is not, so that an infinite value
+  // stays infinite (the sum of its products would otherwise hold inf * 0, or inf and -inf).
+  struct Probs { bf16x8 v, rest; };
   static __device__ __forceinline__ Probs probs(const f32x4 (&p)[2]) {
     Probs o;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      o.v[i] = static_cast<__bf16>(p[i / 4][i % 4]);
-      o.rest[i] = static_cast<__bf16>(p[i / 4][i % 4] - static_cast<float>(o.v[i]));
+      const uint32_t below = __builtin_elementwise_sub_sat(__float_as_uint(p[i / 4][i % 4]), 1u) & 0xffff0000u;
+      o.v[i] = __builtin_bit_cast(__bf16, static_cast<uint16_t>(below >> 16));
+      o.rest[i] = static_cast<__bf16>(p[i / 4][i % 4] - __uint_as_float(below));
     }
     return o;
   }

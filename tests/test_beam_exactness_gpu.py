@@ -15,10 +15,10 @@ BF16 = torch.bfloat16
 
 def check(out, q, k, v, tables, ctx, H, KV, d, scale, sinks=None):
     """A score is off by 2^-24 sqrt(d) of its size, a probability by as much: 2.5e-5 of the sum of |p v| (scores up to 8).  A probability
-    goes into its product as two bf16 numbers: the first is off by at most 2^-8 of it, the second by 2^-8 of that, 2^-16.  What
+    goes into its product as two bf16 numbers: the first is off by at most 2^-7 of it (cut), the second by 2^-8 of that, 2^-15.  What
     is stored is off by 2^-8 of itself."""
     want, weight = plain.attend(q, k, v, tables, ctx, H, KV, d, scale, sinks)
-    inner = (2.5e-5 + 2.0 ** -16) * weight + 1e-7
+    inner = (2.5e-5 + 2.0 ** -15) * weight + 1e-7
     off = (out.cpu().double() - want).abs()
     bound = inner + 2.0 ** -8 * (want.abs() + inner)
     assert bool((off <= bound).all()), float((off - bound).max())
@@ -42,3 +42,21 @@ def test_bf16_outputs_of_any_pages_and_cuts(page, cuts):
     q = torch.randn(len(ctx), 6 * 48, generator=torch.Generator().manual_seed(page)).to(BF16)
     out = run_attend(q, k, v, tables, cu, shared, ctx, 6, 2, 48, 0.2, cuts=cuts)
     check(out, q, k, v, tables, ctx, 6, 2, 48, 0.2)
+
+
+@pytest.mark.parametrize("d", [16, 64, 128])
+def test_a_value_that_is_infinite_stays_infinite(d):
+    """Where a sequence sees it; two of unlike signs are no number, and neither reaches other elements or sequences."""
+    H, KV = 4, 2
+    k, v, tables, cu, shared, ctx = paged([(64, [70, 90, 66])], KV, d, 16, BF16, 9)
+    q = torch.randn(3, H * d, generator=torch.Generator().manual_seed(4)).to(BF16)
+    v[tables[0][0], 0, 3, 5] = float("inf")                        # a shared key
+    v[tables[0][1], 1, 7, 2] = float("-inf")
+    v[tables[0][2], 0, 9, 0], v[tables[0][3], 0, 9, 15] = float("inf"), float("-inf")
+    v[tables[1][4], 0, 4, 3] = float("inf")                        # one of the second sequence's own
+    out = run_attend(q, k, v, tables, cu, shared, ctx, H, KV, d, d ** -0.5).cpu().float().view(3, H, d)
+    want, _ = plain.attend(q, k, v, tables, ctx, H, KV, d, d ** -0.5)
+    want = want.view(3, H, d)
+    assert want[0, 0, 3] == float("inf") and want[1, 3, 7] == float("-inf") and want[2, 1, 9].isnan() and want[1, 0, 4] == float("inf")
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out == float("inf"), want == float("inf"))
+    assert torch.equal(out == -float("inf"), want == -float("inf"))

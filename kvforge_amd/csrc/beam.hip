@@ -137,7 +137,9 @@ struct PieceArgs {
 };
 
 // sums[row][piece] = (sum of exponentials, their reference), values/tokens[row][piece][count]: sorted, token -1 behind the last.
-// RULED: the sum is made first, from the same logits in the same order, then the tokens in `ruled` leave the registers.
+// RULED: the sum is made first, from the same logits in the same order, then the tokens in `ruled` leave the registers: a bit for each
+// logit of the piece, set by whatever thread comes to the token (or-ing has no order).  4 rows of 8,192, 8 best: 8.6, 8.6, 9.0 us with 2, 43
+// and 1,000 tokens, 8.2 without; 512 rows of 128,256, 16 best: 58.9, 59.1, 65.0, 52.0 without.
 template <typename T, int E, bool RULED>
 __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restrict__ logits, const float* __restrict__ scores,
                                                               double2* __restrict__ sums, float* __restrict__ values,
@@ -210,20 +212,26 @@ __global__ __launch_bounds__(THREADS) void beam_pieces_kernel(const T* __restric
     s = wave_sum64(s);
   };
   if constexpr (RULED) {
+    __shared__ uint32_t out_bits[THREADS * E / 32];
     const float wmx = wave_most(mx);
     if (lane == 0) max_of[wave] = wmx;
+    if (tid < THREADS * E / 32) out_bits[tid] = 0u;
+    static_assert(E <= 32, "a word a thread at most");
     __syncthreads();
+    for (int k = tid; k < a.n_ruled; k += THREADS) {
+      const int token = ruled[k];
+      if (token >= 0 && token >= lo && token < hi) atomicOr(&out_bits[(token - lo) / 32], 1u << ((token - lo) % 32));
+    }
 #pragma unroll
     for (int w = 0; w < NWAVES; ++w) m = fmaxf(m, max_of[w]);
     sum_up();
-    for (int k = 0; k < a.n_ruled; ++k) {
-      const int token = ruled[k];           // (the same for the whole workgroup)
-      if (token < lo || token < 0 || token >= hi) continue;
+    __syncthreads();
 #pragma unroll
-      for (int c = 0; c < CHUNKS; ++c)
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int at0 = (c * THREADS + tid) * N;
+      const uint32_t out = out_bits[at0 / 32] >> (at0 % 32);
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (lo + (c * THREADS + tid) * N + i == token) v[c][i] = -INFINITY;
+      for (int i = 0; i < N; ++i) v[c][i] = out >> i & 1u ? -INFINITY : v[c][i];
     }
     mx = -INFINITY;
 #pragma unroll

@@ -24,9 +24,11 @@
 // up to 5 beams behind up to 2,900 keys), and 0.2% where the bytes do.
 //
 // What bounds it: the keys' bytes where there are many of them (4 x 8 beams behind 32,768 keys, 8 kv heads of 128, bf16: 552 MB in
-// 106 us, 5.2 TB/s, about what a kernel that only reads reaches), otherwise the chain of loads that a workgroup begins with
-// (group, lengths, page, K, V) and the second launch: 7 us for 4 beams behind 300 keys.  Against one pass per sequence, which
-// reads shared keys once a beam: 16 x 8 beams behind 4,096 keys, heads of 128, 47 us and 167, heads of 64, 27 and 79.
+// 105 us, 5.3 TB/s, about what a kernel that only reads reaches), otherwise the chain of loads that a workgroup begins with
+// (group, lengths, page, K, V) and the second launch: 7 us for 4 beams behind 300 keys; in between, units without a share of
+// the keys (12 x 16 beams of 24 heads of 128 behind 1,777: 192 workgroups walk the shared keys on 256 units, 43 us for 142 MB; fp32
+// 288 on 256 units that hold one each, 94 us for 284 MB).  Against one pass per sequence, which
+// reads shared keys once a beam: 16 x 8 beams behind 4,096 keys, heads of 128, 47 us and 166, heads of 64, 28 and 79.
 #include <type_traits>
 
 #include "common.h"
@@ -40,7 +42,7 @@ constexpr float LAZY = 8.f;
 constexpr float LOG2E = 1.4426950408889634f;
 
 // Where two waves a SIMD are asked for, a wave has at most 256 registers.  (fp32 heads of 128 need a few more: 12 x 16 beams
-// behind 1,777 keys, 24 heads, 106 us with spills, 95 with one wave a SIMD; heads of 64 in two tiles fit, 63 and 64.)
+// behind 1,777 keys, 24 heads, 106 us with spills, 94 with one wave a SIMD; heads of 64 in two tiles fit, 63 and 64.)
 #define KVF_TWO_WAVES(FITS) __attribute__((amdgpu_waves_per_eu((FITS) ? 2 : 1)))
 
 struct Args {
@@ -255,8 +257,8 @@ template <typename T, int DT, int RT, Form FORM> struct Rows {
           for (int c = 0; c < SLICES; ++c) s[rt][tt] = F::scores(within(kf[tt][c], c * F::SLICE + g * LANE_D, d), q[rt][c], s[rt][tt]);
         }
       if constexpr (more) load_k(next, pk_next);
-      // All products are read here, ahead of any branch: hipcc 7.2 puts no wait between a product of the matrix cores and the
-      // first read of it in a block where a branch around a long one meets the long one.
+      // All products are read here, ahead of any branch: in a form of this loop where the first read of a product of the matrix cores
+      // stood behind the meeting of two branches, one of them long, hipcc 7.2 put no wait ahead of it, and scores were wrong.
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll

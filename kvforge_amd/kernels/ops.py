@@ -1766,7 +1766,9 @@ def attn_beams_cuts(q: torch.Tensor, k_pages: torch.Tensor, num_heads: int, num_
     Measured, us, with half, three quarters, one, twice that of the compute units: one tile, 2 x 4 beams behind 8,192 keys
     (heads of 128, bf16) 17.9, 17.1, 18.8, 20.8, 8 x 4 behind 2,048 (64, fp32) 20.0, 18.4, 20.0, 21.5; two, 4 x 8 behind 32,768
     (128, bf16) 124, 106, 104, 106, 8 x 8 behind 4,096 (64, fp32) 47, 38, 32, 33, 8 x 5 behind up to 2,900 (64, bf16) 14.9, 13.7,
-    12.6, 12.7.  ``max_shared``, ``max_own``: the most shared keys of a group and own keys of a sequence (any cuts give right
+    12.6, 12.7.  Cuts are whole and the same for all groups, so units are left over where there are not many items: 192 items of two
+    tiles (12 x 16 beams, 24 heads over 8 kv heads) are one cut each, and a quarter of 256 units has no part in the shared keys; and the
+    longest of uneven groups takes as few cuts as the others.  ``max_shared``, ``max_own``: the most shared keys of a group and own keys of a sequence (any cuts give right
     results for any lengths)."""
     units = compute_units(q.device)
     rows = max(1, widest) * (num_heads // num_kv_heads)
@@ -2999,7 +3001,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, cu_beams: torch.Tens
 class CacheRows:
     """Tensors whose rows (pages, or state slots, of every layer) move together: ``beam_reorder`` moves the same rows in all
     of them with one launch.  Rows are dense; they may be columns of wider ones.  Keeps the tensors, and a table of the pieces
-    of their rows on their device."""
+    of their rows on their device.  Made once for tensors that stay: checking them and building the table takes the host 0.2 ms for
+    64 tensors, more than a reordering of them takes."""
 
     def __init__(self, tensors) -> None:
         self.tensors = list(tensors)

@@ -28,10 +28,10 @@ from kvforge_amd.registry import register_mixer
 KEYS_PER_CUT = 512
 MAX_CUTS = 64            # what the merge kernels take
 SKEW_MAX_CUTS = 8
-# Sequences that share their first pages go to the kernel that reads these once a group from so many shared keys on (against
-# the kernel that reads every sequence's by themselves: bf16, heads of 64, one request of 4 beams, 512 shared keys 7.1 and 6.9
-# us, 1,024 7.2 and 9.8; 16 of 8 beams, 256 shared keys 9.6 and 11.5, 4,096 27 and 79).  In 32 bits always (4 beams, 16 keys 7.9
-# and 10.5, 4,096 10.6 and 30.8).
+# Sequences that share their first pages go to the kernel that reads these once a group behind more than so many shared keys
+# (counted in cells of 512, so from 513 on), against the kernel that reads every sequence's by themselves: bf16, heads of 64,
+# one request of 4 beams, 512 shared keys 7.3 and 7.0 us, 1,024 7.3 and 9.7; 16 of 8 beams, 256 shared keys 9.8 and 11.5, 4,096
+# 28 and 79.  In 32 bits always (4 beams, 16 keys 7.9 and 10.6, 4,096 10.7 and 31.3).
 SHARED_FROM = 512
 
 

@@ -1,7 +1,9 @@
-"""bf16 attention behind shared pages is off by no more than its inputs' type asks: sums as exact as in 32 bits, and the one rounding of
-what is stored."""
+"""Attention behind shared pages is off by no more than its inputs' type asks: in bf16 sums as exact as in 32 bits, and the one rounding of
+what is stored; in 32 bits scores that lose no more than a sum in a few runs does."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -60,3 +62,24 @@ def test_a_value_that_is_infinite_stays_infinite(d):
     assert want[0, 0, 3] == float("inf") and want[1, 3, 7] == float("-inf") and want[2, 1, 9].isnan() and want[1, 0, 4] == float("inf")
     assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out == float("inf"), want == float("inf"))
     assert torch.equal(out == -float("inf"), want == -float("inf"))
+
+
+@pytest.mark.parametrize("H,KV", [(1, 1), (20, 2)])
+@pytest.mark.parametrize("d", [96, 128, 192, 256])
+def test_32_bit_scores_are_summed_in_runs(H, KV, d):
+    """A score of 2^11 from one element and a last run of elements whose products are each a quarter of 0.9 half steps of it: added one after
+    the other to 2^11 they are lost, four at a time too; summed by themselves first they are there.  Two keys, one with them and one
+    without, values 1 and -1: the output is tanh of half their scores' difference.  A score is rounded by half a step (2^-13), and so is
+    its product with log2(e) (2^-13 again, ln 2 of it in the exponent), for both keys: 2^-13 (1 + 2 ln 2) of the difference at
+    most, half of that in the output, 1.46e-4.  What was lost is 0.9 * n / 4 half steps, n = 32 at least: 4.4e-4."""
+    first = {96: 64, 128: 64, 192: 128, 256: 128}[d]
+    k, v = torch.zeros(1, KV, 16, d), torch.zeros(1, KV, d, 16)
+    k[0, :, :2, 0] = 2.0 ** 11
+    k[0, :, 0, first:] = 0.9 * 2.0 ** -15
+    v[0, :, :, 0], v[0, :, :, 1] = 1.0, -1.0
+    q = torch.zeros(2, H, d)
+    q[:, :, 0], q[:, :, first:] = 1.0, 1.0
+    for shared in (0, 2):
+        out = run_attend(q.view(2, H * d), k, v, [[0], [0]], [0, 2], [shared], [2, 2], H, KV, d, 1.0).cpu().double()
+        want, _ = plain.attend(q.view(2, H * d), k, v, [[0], [0]], [2, 2], H, KV, d, 1.0)
+        assert bool((out - want).abs().max() <= 2.0 ** -13 * (0.5 + math.log(2.0))), (out[0, 0], want[0, 0])

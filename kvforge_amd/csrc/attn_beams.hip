@@ -20,8 +20,9 @@
 // A row's reference (what is subtracted in the exponent) is raised only when a score passes it by LAZY (in log2 units); scores,
 // sums and accumulators are fp32.  bf16: a probability enters its product with V as the sum of two bf16 numbers, itself cut and
 // what that leaves, 2^-15 of it off: outputs are off by the rounding of what is stored (0.0017 of their largest; rounded once,
-// probabilities alone would make that up to 0.0025).  The second products take 0.5 of 13.7 us where the chain of a few blocks bounds (8 x
-// up to 5 beams behind up to 2,900 keys), and 0.2% where the bytes do.
+// probabilities alone would make that up to 0.0025).  Splitting them and the second products take 0.4 of 13.5 us where the chain of a
+// few blocks bounds (8 x up to 5 beams behind up to 2,900 keys), 2 of 23.5 where the vector units do most (two tiles of rows of
+// heads of 64, 6 x up to 12 behind up to 5,181), and 0.3% where the bytes bound.
 //
 // What bounds it: the keys' bytes where there are many of them (4 x 8 beams behind 32,768 keys, 8 kv heads of 128, bf16: 552 MB in
 // 105 us, 5.3 TB/s, about what a kernel that only reads reaches), otherwise the chain of loads that a workgroup begins with
@@ -74,16 +75,16 @@ template <> struct Frag<bf16_t> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) k.v[i] = keep >> i & 1u ? k.v[i] : static_cast<__bf16>(0.f);
   }
-  // v + rest, v the largest bf16 number below the probability: neither is zero where the probability is not, so that an infinite value
-  // stays infinite (the sum of its products would otherwise hold inf * 0, or inf and -inf).
+  // v + rest, v the probability cut to bf16.  The rest of 1 + 2^-23 of it is positive where the probability is, so that an infinite
+  // value stays infinite (the sum of its products would otherwise hold inf * 0, or inf and -inf).
   struct Probs { bf16x8 v, rest; };
   static __device__ __forceinline__ Probs probs(const f32x4 (&p)[2]) {
     Probs o;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t below = __builtin_elementwise_sub_sat(__float_as_uint(p[i / 4][i % 4]), 1u) & 0xffff0000u;
-      o.v[i] = __builtin_bit_cast(__bf16, static_cast<uint16_t>(below >> 16));
-      o.rest[i] = static_cast<__bf16>(p[i / 4][i % 4] - __uint_as_float(below));
+      const uint32_t cut = __float_as_uint(p[i / 4][i % 4]) & 0xffff0000u;
+      o.v[i] = __builtin_bit_cast(__bf16, static_cast<uint16_t>(cut >> 16));
+      o.rest[i] = static_cast<__bf16>(fmaf(p[i / 4][i % 4], 1.f + 0x1p-23f, -__uint_as_float(cut)));
     }
     return o;
   }
